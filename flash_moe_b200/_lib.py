@@ -20,6 +20,7 @@ DTYPE_CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 NUM_STAGES = 6
 STAGE_NAMES = ("router_front", "router_topk", "expert_scores", "expert_accum", "mlp_up", "mlp_down")
 
+ERR_BAD_ARG = 1  # fmoe_error: null pointer, negative size, ...
 ERR_UNSUPPORTED = 2  # fmoe_error: a shape/dtype combination no kernel covers
 ERR_ALIGNMENT = 4  # fmoe_error: pointer or row pitch not 16-byte aligned
 STATUS_BAD_EXPERT_ID = 1
@@ -115,6 +116,18 @@ SIGNATURES = {
     "fmoe_dense_backward_f32": (_I, [ctypes.c_char_p]),
     "fmoe_gather_probe": (_I, [_P, _L, _P, _L, _I, _I, _I, _P, _P, _P]),
     "fmoe_rms_norm": (_I, [_P, _P, _P, _I, _L, _I, _F, _P]),
+    "fmoe_add_rms_norm": (_I, [_P, _P, _P, _P, _P, _I, _L, _I, _F, _P]),
+    "fmoe_add_rms_norm_fp8": (_I, [_P, _P, _P, _P, _P, _P, _I, _L, _I, _I, _F, _P]),
+    "fmoe_add_rms_norm_backward_workspace_bytes": (_Z, [_L, _I, _I]),
+    "fmoe_add_rms_norm_backward": (_I, [_P, _P, _P, _P, _P, _P, _I, _L, _I, _F, _P, _Z, _P]),
+    "fmoe_grad_norm_workspace_bytes": (_Z, [_I]),
+    "fmoe_grad_norm": (_I, [_P, _P, _P, _I, _F, _P, _P, _P, _Z, _P]),
+    "fmoe_clip_grad_norm": (_I, [_P, _P, _P, _I, _F, _F, _F, _P, _P, _P, _Z, _P]),
+    "fmoe_expert_counts": (_I, [_P, _P, _L, _I, _L, _P, _P, _P]),
+    "fmoe_balance_loss_prepared_bytes": (_Z, [_I]),
+    "fmoe_balance_loss_workspace_bytes": (_Z, [_L]),
+    "fmoe_balance_loss_forward": (_I, [_P, _L, _L, _I, _P, _P, _L, _I, _P, _P, _P, _Z, _P, _Z, _P]),
+    "fmoe_balance_loss_backward": (_I, [_P, _L, _L, _I, _P, _L, _I, _P, _P, _Z, _P, _P, _P]),
     "fmoe_selftest_wait_timeout": (_I, [ctypes.c_uint64, _P, _P, _P]),
     "fmoe_combine_partial_rows": (_I, [_P, _L, _P, _I, _L, _I, _P, _P, _P]),
     "fmoe_expert_workspace_bytes": (_Z, [_L, _I, _L, _I]),

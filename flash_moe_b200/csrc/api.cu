@@ -377,6 +377,72 @@ int fmoe_rms_norm(const void* x, const void* weight, void* out, int dtype, int64
   return launch_rms_norm(x, weight, out, dtype, num_tokens, hidden, eps, static_cast<cudaStream_t>(stream));
 }
 
+int fmoe_add_rms_norm(const void* x, const void* residual, const void* weight, void* summed, void* normed, int dtype,
+                      int64_t num_tokens, int hidden, float eps, fmoe_stream_t stream) {
+  if (!valid_dtype(dtype)) return FMOE_ERR_BAD_ARG;
+  return launch_add_rms_norm(x, residual, weight, summed, normed, nullptr, nullptr, dtype, num_tokens, hidden, 0, eps,
+                             static_cast<cudaStream_t>(stream));
+}
+
+int fmoe_add_rms_norm_fp8(const void* x, const void* residual, const void* weight, void* summed, void* q, float* scales,
+                          int dtype, int64_t num_tokens, int hidden, int group, float eps, fmoe_stream_t stream) {
+  if (!valid_dtype(dtype) || (num_tokens > 0 && (q == nullptr || scales == nullptr))) return FMOE_ERR_BAD_ARG;
+  return launch_add_rms_norm(x, residual, weight, summed, nullptr, q, scales, dtype, num_tokens, hidden, group, eps,
+                             static_cast<cudaStream_t>(stream));
+}
+
+size_t fmoe_add_rms_norm_backward_workspace_bytes(int64_t num_tokens, int hidden, int dtype) {
+  return valid_dtype(dtype) ? add_rms_norm_backward_workspace_bytes(num_tokens, hidden, dtype) : 0;
+}
+
+int fmoe_add_rms_norm_backward(const void* dnormed, const void* dsummed, const void* summed, const void* weight, void* dx,
+                               void* dweight, int dtype, int64_t num_tokens, int hidden, float eps, void* workspace,
+                               size_t workspace_bytes, fmoe_stream_t stream) {
+  if (!valid_dtype(dtype)) return FMOE_ERR_BAD_ARG;
+  return launch_add_rms_norm_backward(dnormed, dsummed, summed, weight, dx, dweight, dtype, num_tokens, hidden, eps, workspace,
+                                      workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+size_t fmoe_grad_norm_workspace_bytes(int num_tensors) { return grad_norm_workspace_bytes(num_tensors); }
+
+int fmoe_grad_norm(void* const* grads, const int64_t* numels, const int32_t* dtypes, int num_tensors, float scale,
+                   const float* device_scale, float* norm, void* workspace, size_t workspace_bytes, fmoe_stream_t stream) {
+  return launch_grad_norm(grads, numels, dtypes, num_tensors, false, 0.f, 0.f, scale, device_scale, norm, workspace, workspace_bytes,
+                          static_cast<cudaStream_t>(stream));
+}
+
+int fmoe_clip_grad_norm(void* const* grads, const int64_t* numels, const int32_t* dtypes, int num_tensors, float max_norm, float eps,
+                        float scale, const float* device_scale, float* norm, void* workspace, size_t workspace_bytes,
+                        fmoe_stream_t stream) {
+  return launch_grad_norm(grads, numels, dtypes, num_tensors, true, max_norm, eps, scale, device_scale, norm, workspace,
+                          workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int fmoe_expert_counts(const int64_t* indices, const uint8_t* token_mask, int64_t num_tokens, int top_k, int64_t num_experts,
+                       int64_t* counts, int32_t* status, fmoe_stream_t stream) {
+  return launch_expert_counts(indices, token_mask, num_tokens, top_k, num_experts, counts, status, static_cast<cudaStream_t>(stream));
+}
+
+size_t fmoe_balance_loss_prepared_bytes(int num_keys) { return balance_prepared_bytes(num_keys); }
+size_t fmoe_balance_loss_workspace_bytes(int64_t num_tokens) { return balance_workspace_bytes(num_tokens); }
+
+int fmoe_balance_loss_forward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, const int64_t* counts,
+                              const uint8_t* token_mask, int64_t num_tokens, int num_keys, float* loss, float* token_stats,
+                              void* prepared, size_t prepared_bytes, void* workspace, size_t workspace_bytes,
+                              fmoe_stream_t stream) {
+  if (!valid_dtype(dtype)) return FMOE_ERR_BAD_ARG;
+  return launch_balance_forward(logits, token_stride, half_stride, dtype, counts, token_mask, num_tokens, num_keys, loss, token_stats,
+                                prepared, prepared_bytes, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+int fmoe_balance_loss_backward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, const uint8_t* token_mask,
+                               int64_t num_tokens, int num_keys, const float* token_stats, const void* prepared,
+                               size_t prepared_bytes, const float* upstream, void* dlogits, fmoe_stream_t stream) {
+  if (!valid_dtype(dtype)) return FMOE_ERR_BAD_ARG;
+  return launch_balance_backward(logits, token_stride, half_stride, dtype, token_mask, num_tokens, num_keys, token_stats, prepared,
+                                 prepared_bytes, upstream, dlogits, static_cast<cudaStream_t>(stream));
+}
+
 int fmoe_combine_partial_rows(const float* rows, int64_t num_rows, const int32_t* slot, int num_sources,
                               int64_t num_tokens, int hidden, float* out, int32_t* status, fmoe_stream_t stream) {
   return launch_combine_rows(rows, num_rows, slot, num_sources, num_tokens, hidden, out, status,

@@ -295,6 +295,29 @@ int launch_gather_probe(const void* table, int64_t num_rows, const int32_t* row_
                         int ctas_per_sm, int mode, float* sink, int32_t* status, cudaStream_t stream);
 int launch_rms_norm(const void* x, const void* weight, void* out, int dtype, int64_t ntok, int H, float eps,
                     cudaStream_t stream);
+// add_rms_norm.cu: q and scales for the 8-bit output, normed for the other
+int launch_add_rms_norm(const void* x, const void* residual, const void* weight, void* summed, void* normed, void* q,
+                        float* scales, int dtype, int64_t rows, int H, int group, float eps, cudaStream_t stream);
+size_t add_rms_norm_backward_workspace_bytes(int64_t rows, int H, int dtype);
+int launch_add_rms_norm_backward(const void* dnormed, const void* dsummed, const void* summed, const void* weight, void* dx,
+                                 void* dweight, int dtype, int64_t rows, int H, float eps, void* ws, size_t ws_bytes,
+                                 cudaStream_t stream);
+// grad_clip.cu: clip == false leaves the gradients alone
+size_t grad_norm_workspace_bytes(int count);
+int launch_grad_norm(void* const* grads, const int64_t* numels, const int32_t* dtypes, int count, bool clip, float max_norm,
+                     float eps, float scale, const float* device_scale, float* norm, void* ws, size_t ws_bytes,
+                     cudaStream_t stream);
+// balance.cu
+int launch_expert_counts(const int64_t* indices, const uint8_t* mask, int64_t T, int k, int64_t N, int64_t* counts, int32_t* status,
+                         cudaStream_t stream);
+size_t balance_prepared_bytes(int nk);
+size_t balance_workspace_bytes(int64_t T);
+int launch_balance_forward(const void* logits, int64_t ts, int64_t hs, int dtype, const int64_t* counts, const uint8_t* mask, int64_t T,
+                           int nk, float* loss, float* token_s, void* prepared, size_t prepared_bytes, void* ws, size_t ws_bytes,
+                           cudaStream_t stream);
+int launch_balance_backward(const void* logits, int64_t ts, int64_t hs, int dtype, const uint8_t* mask, int64_t T, int nk,
+                            const float* token_s, const void* prepared, size_t prepared_bytes, const float* upstream, void* dlogits,
+                            cudaStream_t stream);
 int launch_combine_rows(const float* rows, int64_t num_rows, const int32_t* slot, int num_sources, int64_t ntok, int H,
                         float* out, int32_t* status, cudaStream_t stream);
 

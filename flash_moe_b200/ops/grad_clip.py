@@ -1,0 +1,92 @@
+"""Global norm of gradients and clipping: the layer's backward writes dense gradients of both expert tables, so the pass over them
+is one of the longer ones of a training step (the reference leaves it to its caller)."""
+
+from __future__ import annotations
+
+from array import array
+from typing import Iterable, List, Union
+
+import torch
+
+from .. import _lib
+
+
+def _dense(t: torch.Tensor) -> bool:
+    """True where the tensor's values are one stretch of memory without gaps or repeats, in any order of its dimensions."""
+    if t.is_contiguous():
+        return True
+    step = 1
+    for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n != 1):
+        if stride != step:
+            return False
+        step *= size
+    return True
+
+
+def _call(name, grads: List[torch.Tensor], head, grad_scale) -> torch.Tensor:
+    dev = _lib.require_cuda(*grads)
+    scale, device_scale = grad_scale, None
+    if isinstance(grad_scale, torch.Tensor):
+        if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
+            raise _lib.FmoeError("a grad_scale tensor must hold one float32 value on the device of the gradients")
+        scale, device_scale = 1.0, grad_scale.data_ptr()
+    elif not 0 <= grad_scale < float("inf"):
+        raise _lib.FmoeError("grad_scale must be a finite number that is not negative")
+    n = len(grads)
+    ptrs = array("Q", [g.data_ptr() for g in grads])
+    numels = array("q", [g.numel() for g in grads])
+    codes = array("i", [_lib.dtype_code(g) for g in grads])
+    norm = torch.empty((), dtype=torch.float32, device=dev)
+    nbytes = _lib.lib().fmoe_grad_norm_workspace_bytes(n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    rc = _lib.call(name, dev, ptrs.buffer_info()[0], numels.buffer_info()[0], codes.buffer_info()[0], n, *head, scale, device_scale,
+                   norm.data_ptr(), ws.data_ptr(), nbytes)
+    if rc == _lib.ERR_BAD_ARG:
+        raise _lib.FmoeError("two gradients share memory")
+    if rc:
+        _lib.check(rc, name)
+    return norm
+
+
+def _once(tensors: Iterable[torch.Tensor]) -> List[torch.Tensor]:
+    """Each tensor that has values once, however often it is given."""
+    seen = {}
+    for t in tensors:
+        if t.is_sparse or t.layout != torch.strided:
+            raise _lib.FmoeError("sparse gradients are not supported")
+        if t.numel():
+            seen.setdefault((t.data_ptr(), t.numel(), t.dtype), t)
+    return list(seen.values())
+
+
+def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], grad_scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
+    """``grad_scale * sqrt(sum of all squares)`` over all tensors, a float32 scalar on their device (no synchronisation).  A tensor
+    given twice counts once."""
+    tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    grads = _once(t.detach() for t in tensors)
+    if not grads:
+        return torch.zeros((), device=tensors[0].device if tensors else None)
+    return _call("fmoe_grad_norm", [g if _dense(g) else g.contiguous() for g in grads], (), grad_scale)
+
+
+def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float,
+                    grad_scale: Union[float, torch.Tensor] = 1.0, eps: float = 1e-6) -> torch.Tensor:
+    """Scale the gradients of `parameters` in place so that their global 2-norm is at most `max_norm`; returns that norm before
+    clipping, a float32 scalar on their device (no synchronisation).
+
+    With ``n = grad_scale * sqrt(sum of all squares)`` every gradient is multiplied by ``grad_scale * min(1, max_norm / (n + eps))``
+    in float32 and rounded once; where that factor is 1 nothing is written.  `grad_scale` is a number or one float32 on the device:
+    the inverse of a loss scale, or the number of ranks where averaged gradients are to be summed.  Parameters without a gradient
+    are left out, one given twice counts once.  float32, bfloat16 and float16 gradients may be mixed; each must be dense, and all on
+    one device."""
+    parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    if not max_norm >= 0 or not eps >= 0:
+        raise _lib.FmoeError("max_norm and eps must not be negative")
+    grads = _once(p.grad for p in parameters if p.grad is not None)
+    if not grads:
+        return torch.zeros((), device=parameters[0].device if parameters else None)
+    if not all(_dense(g) for g in grads):
+        raise _lib.FmoeError("a gradient with gaps or repeated values cannot be scaled in place: make it contiguous")
+    norm = _call("fmoe_clip_grad_norm", grads, (max_norm, eps), grad_scale)
+    torch.autograd.graph.increment_version(grads)
+    return norm

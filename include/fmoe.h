@@ -200,6 +200,70 @@ int fmoe_rms_norm(const void* x, const void* weight, void* out, int dtype, int64
                   fmoe_stream_t stream);
 
 /*
+ * The same norm behind the residual's addition, with its gradient and with an output in 8 bits (no counterpart in the reference;
+ * Python: flash_moe_b200.ops.add_rms_norm).  With s = dtype(x + residual):
+ *   fmoe_add_rms_norm           summed = s, normed = dtype(s * rsqrt(mean(s^2) + eps) * weight)
+ *   fmoe_add_rms_norm_fp8       summed = s, and the float32 value y of the norm in 8 bits: scales = max(max |y| / 448, 2^-126) over
+ *                               each row (group 0) or each `group` = 32, 64 or 128 columns of it ([T, ceil(H / group)], the last
+ *                               block may be short), q [T, H] = e4m3(y / scale).  A value that is not finite makes its scale so
+ *   fmoe_add_rms_norm_backward  from dnormed and dsummed (nullable) the gradient dx of both x and residual, and dweight
+ *                               (nullable): sums in float32 in a fixed order, one rounding
+ * residual (nullable, then summed is null too: x itself is normalised), weight (nullable) [hidden].  hidden is at most 16384, any
+ * number; rows of aligned 16-byte pieces are read in those.
+ */
+int fmoe_add_rms_norm(const void* x, const void* residual, const void* weight, void* summed, void* normed, int dtype,
+                      int64_t num_tokens, int hidden, float eps, fmoe_stream_t stream);
+int fmoe_add_rms_norm_fp8(const void* x, const void* residual, const void* weight, void* summed, void* q, float* scales,
+                          int dtype, int64_t num_tokens, int hidden, int group, float eps, fmoe_stream_t stream);
+size_t fmoe_add_rms_norm_backward_workspace_bytes(int64_t num_tokens, int hidden, int dtype);
+int fmoe_add_rms_norm_backward(const void* dnormed, const void* dsummed, const void* summed, const void* weight, void* dx,
+                               void* dweight, int dtype, int64_t num_tokens, int hidden, float eps, void* workspace,
+                               size_t workspace_bytes, fmoe_stream_t stream);
+
+/*
+ * Global norm of gradients and clipping (no counterpart in the reference; Python: flash_moe_b200.ops.grad_clip).
+ *   fmoe_grad_norm       *norm = scale * sqrt(sum over all values g^2)
+ *   fmoe_clip_grad_norm  the same, then in place g <- g * scale * min(1, max_norm / (*norm + eps)); nothing is written where that
+ *                        factor is 1.  A norm that is not finite makes the gradients so, or zero them, as the formula says
+ * grads, numels and dtypes are HOST arrays of num_tensors entries, grads device pointers to dense tensors of any alignment, no
+ * two of which may share memory.  scale >= 0; device_scale (nullable, one float in device memory) multiplies it: the inverse of
+ * a loss scale.  Squares and products in float32, the sum over 16 KiB pieces in float64, in a fixed order.
+ */
+size_t fmoe_grad_norm_workspace_bytes(int num_tensors);
+int fmoe_grad_norm(void* const* grads, const int64_t* numels, const int32_t* dtypes, int num_tensors, float scale,
+                   const float* device_scale, float* norm, void* workspace, size_t workspace_bytes, fmoe_stream_t stream);
+int fmoe_clip_grad_norm(void* const* grads, const int64_t* numels, const int32_t* dtypes, int num_tensors, float max_norm, float eps,
+                        float scale, const float* device_scale, float* norm, void* workspace, size_t workspace_bytes,
+                        fmoe_stream_t stream);
+
+/*
+ * How often each expert was selected (no counterpart in the reference; Python: flash_moe_b200.ops.balance): counts [num_experts]
+ * of indices [T, top_k]; -1 marks an empty slot, other ids outside [0, num_experts) are left out and flagged in *status.
+ * token_mask (nullable) [T], one byte a token: the slots of tokens with 0 are left out.
+ */
+int fmoe_expert_counts(const int64_t* indices, const uint8_t* token_mask, int64_t num_tokens, int top_k, int64_t num_experts,
+                       int64_t* counts, int32_t* status, fmoe_stream_t stream);
+
+/*
+ * Balance loss of the product-key router (no counterpart in the reference, which returns the router's logits for it,
+ * flash_moe/modules/flash_moe.py:103-105; Python: flash_moe_b200.ops.balance).  p_h = softmax(logits[h]), C [num_keys, num_keys] the
+ * first num_keys^2 entries of counts (not negative):
+ *   *loss = num_keys^2 sum_ij (C_ij / sum C) mean_t p_0[t,i] p_1[t,j],  the mean over the tokens of token_mask (nullable: all);
+ *   dlogits [T, 2, num_keys] = its gradient times *upstream (one float in device memory), rows of masked tokens zero.
+ * The loss is 0, and so is its gradient, where there is no selection or no token.  Value i of token t and half h of the logits is at
+ * logits[t * token_stride + h * half_stride + i].  The forward leaves token_stats [T] and `prepared` for the backward.
+ */
+size_t fmoe_balance_loss_prepared_bytes(int num_keys);
+size_t fmoe_balance_loss_workspace_bytes(int64_t num_tokens);
+int fmoe_balance_loss_forward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, const int64_t* counts,
+                              const uint8_t* token_mask, int64_t num_tokens, int num_keys, float* loss, float* token_stats,
+                              void* prepared, size_t prepared_bytes, void* workspace, size_t workspace_bytes,
+                              fmoe_stream_t stream);
+int fmoe_balance_loss_backward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, const uint8_t* token_mask,
+                               int64_t num_tokens, int num_keys, const float* token_stats, const void* prepared,
+                               size_t prepared_bytes, const float* upstream, void* dlogits, fmoe_stream_t stream);
+
+/*
  * Self-test of the bounded device-side waits (no counterpart in the reference): a one-thread kernel waits on a
  * barrier that nothing completes, gives up after limit_ns (clamped to 10 ms), ORs FMOE_STATUS_WAIT_TIMEOUT into
  * *status, writes 2 to *result (1 would mean the barrier completed) and returns; later launches work as usual.
