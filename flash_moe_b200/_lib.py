@@ -125,9 +125,10 @@ SIGNATURES = {
     "fmoe_clip_grad_norm": (_I, [_P, _P, _P, _I, _F, _F, _F, _P, _P, _P, _Z, _P]),
     "fmoe_expert_counts": (_I, [_P, _P, _L, _I, _L, _P, _P, _P]),
     "fmoe_balance_loss_prepared_bytes": (_Z, [_I]),
-    "fmoe_balance_loss_workspace_bytes": (_Z, [_L]),
-    "fmoe_balance_loss_forward": (_I, [_P, _L, _L, _I, _P, _P, _L, _I, _P, _P, _P, _Z, _P, _Z, _P]),
-    "fmoe_balance_loss_backward": (_I, [_P, _L, _L, _I, _P, _L, _I, _P, _P, _Z, _P, _P, _P]),
+    "fmoe_balance_loss_stats_floats": (_Z, [_L, _I]),
+    "fmoe_balance_loss_workspace_bytes": (_Z, [_L, _I]),
+    "fmoe_balance_loss_forward": (_I, [_P, _L, _L, _I, _P, _P, _L, _I, _P, _P, _P, _Z, _P, _Z, _P, _P]),
+    "fmoe_balance_loss_backward": (_I, [_P, _L, _L, _I, _L, _I, _P, _P, _Z, _P, _P, _P, _P]),
     "fmoe_selftest_wait_timeout": (_I, [ctypes.c_uint64, _P, _P, _P]),
     "fmoe_combine_partial_rows": (_I, [_P, _L, _P, _I, _L, _I, _P, _P, _P]),
     "fmoe_expert_workspace_bytes": (_Z, [_L, _I, _L, _I]),

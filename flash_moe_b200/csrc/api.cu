@@ -424,23 +424,24 @@ int fmoe_expert_counts(const int64_t* indices, const uint8_t* token_mask, int64_
 }
 
 size_t fmoe_balance_loss_prepared_bytes(int num_keys) { return balance_prepared_bytes(num_keys); }
-size_t fmoe_balance_loss_workspace_bytes(int64_t num_tokens) { return balance_workspace_bytes(num_tokens); }
+size_t fmoe_balance_loss_stats_floats(int64_t num_tokens, int num_keys) { return balance_stats_floats(num_tokens, num_keys); }
+size_t fmoe_balance_loss_workspace_bytes(int64_t num_tokens, int num_keys) { return balance_workspace_bytes(num_tokens, num_keys); }
 
 int fmoe_balance_loss_forward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, const int64_t* counts,
                               const uint8_t* token_mask, int64_t num_tokens, int num_keys, float* loss, float* token_stats,
-                              void* prepared, size_t prepared_bytes, void* workspace, size_t workspace_bytes,
+                              void* prepared, size_t prepared_bytes, void* workspace, size_t workspace_bytes, int32_t* status,
                               fmoe_stream_t stream) {
   if (!valid_dtype(dtype)) return FMOE_ERR_BAD_ARG;
   return launch_balance_forward(logits, token_stride, half_stride, dtype, counts, token_mask, num_tokens, num_keys, loss, token_stats,
-                                prepared, prepared_bytes, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+                                prepared, prepared_bytes, workspace, workspace_bytes, status, static_cast<cudaStream_t>(stream));
 }
 
-int fmoe_balance_loss_backward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, const uint8_t* token_mask,
-                               int64_t num_tokens, int num_keys, const float* token_stats, const void* prepared,
-                               size_t prepared_bytes, const float* upstream, void* dlogits, fmoe_stream_t stream) {
+int fmoe_balance_loss_backward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, int64_t num_tokens,
+                               int num_keys, const float* token_stats, const void* prepared, size_t prepared_bytes,
+                               const float* upstream, void* dlogits, int32_t* status, fmoe_stream_t stream) {
   if (!valid_dtype(dtype)) return FMOE_ERR_BAD_ARG;
-  return launch_balance_backward(logits, token_stride, half_stride, dtype, token_mask, num_tokens, num_keys, token_stats, prepared,
-                                 prepared_bytes, upstream, dlogits, static_cast<cudaStream_t>(stream));
+  return launch_balance_backward(logits, token_stride, half_stride, dtype, num_tokens, num_keys, token_stats, prepared, prepared_bytes,
+                                 upstream, dlogits, status, static_cast<cudaStream_t>(stream));
 }
 
 int fmoe_combine_partial_rows(const float* rows, int64_t num_rows, const int32_t* slot, int num_sources,

@@ -7,7 +7,16 @@
 //   dlogits[h, t] = upstream (nk^2 / (T sum C)) p_h[t] (G_h[t] - s_t).
 // The rows of p sum to 1, so a constant taken off C shifts G_h and s_t alike: C is used without its (whole) mean, which keeps
 // the bits of the differences where the counts are nearly even.
+//
+// The two products run on the tensor cores (tcgen05) with float16 operands.  A float16 holds 11 bits: each probability, times 2^15,
+// is the sum of two of them to within 2^-24 of it, and so is a count (exactly up to 2^22; up to 2048 the second is zero and its
+// product is left out).  hi C_hi + lo C_hi + hi C_lo in one float32 accumulator is what a float32 product would give.
+//
+// Launches: row statistics (maximum and 1 / sum of both halves) beside the sums of the counts; the centred counts as float16
+// pieces in the order in which shared memory wants them; the product with s_t and the loss; for the gradient one more product
+// kernel, which needs nothing from memory but the logits, five numbers a token and the pieces.
 #include "common.cuh"
+#include "ptx_sm100.cuh"
 
 namespace fmoe {
 namespace {
@@ -24,192 +33,514 @@ __global__ void __launch_bounds__(256) expert_counts_kernel(const int64_t* indic
   }
 }
 
-// What the loss keeps of the counts: one block for both directions.
-struct Prepared {
-  double coef;    // nk^2 / (T sum C), 0 where there is no token or no selection
-  double sum;     // sum C
-  double tokens;  // unmasked
-  float mean;     // what was taken off
-  int pad;
-};
-constexpr int kParts = 64;
+// ------------------------------------------------------------------------------------------------ statistics and counts
+constexpr int kParts = 64;  // CTAs that sum the counts
+constexpr int kMaxKeys = 2048;
+constexpr int kTileTokens = 128;
+constexpr int kChunk = 256;  // columns of a product that one CTA accumulates
+
+inline int padded_keys(int nk) { return (nk + 63) / 64 * 64; }
+inline int column_chunks(int nk) { return (padded_keys(nk) + kChunk - 1) / kChunk; }
+
 struct Part {
-  double sum, tokens;
+  double sum;
+  long long top, tokens;
 };
 
-__global__ void __launch_bounds__(256) balance_sums_kernel(const int64_t* counts, int n, const uint8_t* mask, int64_t T, Part* part) {
-  __shared__ double s[2][8];
-  double c = 0.0, m = 0.0;
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += kParts * 256) c += static_cast<double>(counts[i]);
-  if (mask != nullptr)
-    for (int64_t i = blockIdx.x * 256 + threadIdx.x; i < T; i += kParts * 256) m += mask[i] != 0;
-  for (int d = 16; d > 0; d >>= 1) {
-    c += __shfl_xor_sync(kFull, c, d);
-    m += __shfl_xor_sync(kFull, m, d);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    s[0][threadIdx.x >> 5] = c;
-    s[1][threadIdx.x >> 5] = m;
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) {
-      c += s[0][i];
-      m += s[1][i];
+// What both directions keep of the counts, in front of their pieces.
+struct Prepared {
+  double coef;        // nk^2 / (T sum C), 0 where there is no token or no selection
+  double tokens;      // unmasked
+  float mean;         // what was taken off
+  float unscale;      // accumulator -> G: 2^(shift - 15)
+  int second;         // whether the second pieces of the counts are needed
+  unsigned finished;  // CTAs of the forward product that have ended
+};
+constexpr size_t kHeadBytes = 256;
+
+// (maximum, 1 / sum of exp(x - maximum)) of each half; 0, 0 for masked tokens, which are not read: no sum has an inverse of 0
+template <typename T>
+__global__ void __launch_bounds__(256) balance_stats_kernel(const T* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok,
+                                                            int nk, float4* stats, const int64_t* counts, Part* part) {
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  if (blockIdx.x < kParts) {
+    __shared__ double sums[8];
+    __shared__ long long tops[8], tokens[8];
+    const int n = nk * nk;
+    double c = 0.0;
+    long long top = 0, m = 0;
+    for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += kParts * 256) {
+      const long long v = counts[i];
+      c += static_cast<double>(v);
+      top = v > top ? v : top;
     }
-    part[blockIdx.x] = {c, m};
+    if (mask != nullptr)
+      for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < ntok; i += kParts * 256) m += mask[i] != 0;
+    for (int d = 16; d > 0; d >>= 1) {
+      c += __shfl_xor_sync(kFull, c, d);
+      m += __shfl_xor_sync(kFull, m, d);
+      const long long o = __shfl_xor_sync(kFull, top, d);
+      top = o > top ? o : top;
+    }
+    if (lane == 0) {
+      sums[warp] = c;
+      tops[warp] = top;
+      tokens[warp] = m;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      for (int i = 1; i < 8; ++i) {
+        c += sums[i];
+        m += tokens[i];
+        top = tops[i] > top ? tops[i] : top;
+      }
+      part[blockIdx.x] = {c, top, mask != nullptr ? m : blockIdx.x == 0 ? static_cast<long long>(ntok) : 0ll};
+    }
+  }
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + warp; t < ntok; t += static_cast<int64_t>(gridDim.x) * 8) {
+    float out[4] = {0.f, 0.f, 0.f, 0.f};
+    if (mask == nullptr || mask[t] != 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const T* src = logits + t * ts + h * hs;
+        float top = -INFINITY, sum = 0.f;
+        for (int i = lane; i < nk; i += 32) top = fmaxf(top, to_f32<T>(src[i]));
+        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
+        for (int i = lane; i < nk; i += 32) sum += expf(to_f32<T>(src[i]) - top);
+        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
+        out[2 * h] = top;
+        out[2 * h + 1] = 1.f / sum;
+      }
+    }
+    if (lane == 0) stats[t] = make_float4(out[0], out[1], out[2], out[3]);
   }
 }
 
-__global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* counts, int nk, bool masked, int64_t T, const Part* part,
-                                                              Prepared* head, float* c0, float* c1) {
-  double sum = 0.0, tokens = 0.0;
+// Matrix h [row n][column k]: what multiplies p_(1-h)[k] in G_h[n], so h = 0 is C and h = 1 its transpose.  Stored in blocks of 64
+// columns, [k / 64][n][64], each row 128 bytes with its 16-byte pieces swizzled as the tensor core reads them: a block of rows is
+// copied to shared memory as it is.
+__global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* counts, int nk, int padded, const Part* part, Prepared* head,
+                                                              uint4* pieces) {
+  pdl_launch_dependents();
+  pdl_wait();
+  double sum = 0.0;
+  long long top = 0, tokens = 0;
   for (int i = 0; i < kParts; ++i) {
     sum += part[i].sum;
     tokens += part[i].tokens;
+    top = part[i].top > top ? part[i].top : top;
   }
-  if (!masked) tokens = static_cast<double>(T);
-  const int n = nk * nk;
+  const double n = static_cast<double>(nk) * nk;
   const double mean = rint(sum / n);
+  const double most = fmax(static_cast<double>(top) - mean, mean);
+  int shift = 0;  // the largest value becomes at most 2^15, a float16
+  if (most > 32768.0) shift = ilogb(most) - 14;
+  const bool second = most > 2048.0;
   if (blockIdx.x == 0 && threadIdx.x == 0) {
-    head->coef = sum > 0.0 && tokens > 0.0 ? static_cast<double>(n) / (sum * tokens) : 0.0;
-    head->sum = sum;
-    head->tokens = tokens;
+    head->coef = sum > 0.0 && tokens > 0 ? n / (sum * static_cast<double>(tokens)) : 0.0;
+    head->tokens = static_cast<double>(tokens);
     head->mean = static_cast<float>(mean);
+    head->unscale = static_cast<float>(ldexp(1.0, shift - 15));
+    head->second = second;
+    head->finished = 0;
   }
-  for (int i = blockIdx.x * 256 + threadIdx.x; i < n; i += gridDim.x * 256) {
-    const float v = static_cast<float>(static_cast<double>(counts[i]) - mean);
-    c1[i] = v;                          // [key of half 0][key of half 1]: G_1 reads it along the rows
-    c0[(i % nk) * nk + i / nk] = v;     // transposed, for G_0
+  const double scale = ldexp(1.0, -shift);
+  const int64_t per = static_cast<int64_t>(padded) * padded / 8;  // 16-byte pieces of one matrix
+  const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (at >= 2 * per) return;
+  const int h = at >= per;
+  const int64_t local = at - h * per;
+  int row, col;  // of the matrix; neighbouring threads read neighbouring counts
+  if (h == 0) {
+    row = static_cast<int>(local / (padded / 8));
+    col = static_cast<int>(local % (padded / 8)) * 8;
+  } else {
+    row = static_cast<int>(local % padded);
+    col = static_cast<int>(local / padded) * 8;
   }
-}
-
-constexpr int kTile = 8;  // tokens of a CTA, one warp each for the softmax
-
-// p[h][t][i] of the CTA's tokens, zero for masked ones and behind the last
-template <typename T>
-__device__ void softmax_tile(const T* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t t0, int64_t ntok, int nk, float* p) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  const int64_t t = t0 + w;
-  const bool live = t < ntok && (mask == nullptr || mask[t] != 0);
-  for (int h = 0; h < 2; ++h) {
-    float* row = p + (h * kTile + w) * nk;
-    if (!live) {
-      for (int i = lane; i < nk; i += 32) row[i] = 0.f;
-      continue;
+  float hi[8], lo[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int k = col + i;
+    float v = 0.f, rest = 0.f;
+    if (row < nk && k < nk) {
+      const long long c = h == 0 ? counts[static_cast<int64_t>(row) * nk + k] : counts[static_cast<int64_t>(k) * nk + row];
+      const double d = (static_cast<double>(c) - mean) * scale;
+      v = __half2float(__double2half(d));
+      rest = static_cast<float>(d - static_cast<double>(v));
     }
-    const T* src = logits + t * ts + h * hs;
-    float top = -INFINITY, sum = 0.f;
-    for (int i = lane; i < nk; i += 32) top = fmaxf(top, to_f32<T>(src[i]));
-    for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-    for (int i = lane; i < nk; i += 32) sum += row[i] = expf(to_f32<T>(src[i]) - top);
-    for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-    for (int i = lane; i < nk; i += 32) row[i] /= sum;
+    hi[i] = v;
+    lo[i] = rest;
   }
-  __syncthreads();
+  const int64_t slot = (static_cast<int64_t>(col / 64) * padded + row) * 8 + (((col % 64) / 8) ^ (row & 7));
+  pieces[(2 * h) * per + slot] = pack16<__half>(hi);
+  if (second) pieces[(2 * h + 1) * per + slot] = pack16<__half>(lo);
 }
 
-// g[t] += sum_j c[j][i] p[t][j] for column i of this thread
-__device__ __forceinline__ void product(const float* c, const float* p, int nk, int i, float (&g)[kTile]) {
-  for (int t = 0; t < kTile; ++t) g[t] = 0.f;
-  for (int j = 0; j < nk; ++j) {
-    const float v = c[static_cast<int64_t>(j) * nk + i];
-    for (int t = 0; t < kTile; ++t) g[t] = fmaf(v, p[t * nk + j], g[t]);
-  }
-}
+// ------------------------------------------------------------------------------------------------ product
+// One CTA per SM works through items of 128 tokens x up to 256 columns of G_h (forward: h = 0; backward: both, next to each other
+// so that the second finds the logits in the L2 cache).  Warp roles, each a loop over the items of the CTA:
+//   0      copies the blocks of the counts' pieces into the ring
+//   1      issues the products of a stage: three of 128 x columns x 64, into one of two accumulators
+//   2..5   epilogue, a thread per token: probabilities p_h from the logits, with the accumulator's row
+//   6..13  make the stage's two pieces of p_(1-h), 128 x 64 each, from the logits
+// Every wait is bounded; one that runs out raises FMOE_STATUS_WAIT_TIMEOUT and the CTA drains and leaves.
+constexpr int kMakers = 8;
+constexpr int kProductThreads = (6 + kMakers) * 32;
+constexpr int kPieceBytes = kTileTokens * 128;  // one piece of the probabilities
+constexpr int kMaxStages = 4;
 
-template <typename T>
-__global__ void __launch_bounds__(256) balance_forward_kernel(const T* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok,
-                                                              int nk, const float* c0, float* token_s, double* part) {
-  extern __shared__ float p[];
-  __shared__ float sums[8][kTile];
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  softmax_tile<T>(logits, ts, hs, mask, t0, ntok, nk, p);
-  float s[kTile] = {};
-  for (int i = threadIdx.x; i < nk; i += 256) {
-    float g[kTile];
-    product(c0, p + kTile * nk, nk, i, g);
-    for (int t = 0; t < kTile; ++t) s[t] = fmaf(p[t * nk + i], g[t], s[t]);
-  }
-  for (int t = 0; t < kTile; ++t) {
-    for (int d = 16; d > 0; d >>= 1) s[t] += __shfl_xor_sync(kFull, s[t], d);
-    if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5][t] = s[t];
-  }
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    double all = 0.0;
-    for (int t = 0; t < kTile; ++t) {
-      float v = 0.f;
-      for (int w = 0; w < 8; ++w) v += sums[w][t];
-      if (t0 + t < ntok) token_s[t0 + t] = v;
-      all += v;
+struct ProductArgs {
+  const void* logits;
+  int64_t ts, hs, ntok;
+  const float4* stats;
+  float* token_s;  // [chunks][T]
+  const Prepared* head;
+  const uint4* pieces;
+  double* part;           // forward: [items][4]
+  float* loss;            // forward
+  unsigned* finished;     // forward
+  const float* upstream;  // backward
+  void* dlogits;          // backward: [T, 2, nk]
+  int32_t* status;
+  int nk, padded, chunks, stages;
+  int items;
+};
+
+// eight logits of a row from column c on; `whole`: an aligned piece inside the row
+template <typename T, bool VEC> __device__ __forceinline__ void load_logits(const T* row, int c, int nk, float (&f)[8]) {
+  if constexpr (VEC) {
+    if constexpr (sizeof(T) == 2) {
+      if (c < nk) unpack16<T>(ld16(row + c), *reinterpret_cast<float (*)[Vec16<T>::N]>(&f));
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4)
+        if (c + i < nk) unpack16<T>(ld16(row + c + i), *reinterpret_cast<float (*)[Vec16<T>::N]>(&f[i]));
     }
-    part[blockIdx.x] = all;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (c + i < nk) f[i] = to_f32<T>(row[c + i]);
   }
 }
 
-__global__ void __launch_bounds__(256) balance_loss_kernel(const Prepared* head, const double* part, int64_t parts, float* loss) {
-  __shared__ double sums[8];
-  double v = 0.0;
-  for (int64_t i = threadIdx.x; i < parts; i += 256) v += part[i];
-  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = v;
+__device__ __forceinline__ float probability(float x, float top, float inv) { return __expf(x - top) * inv; }
+
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+template <typename T, bool VEC, bool BACKWARD>
+__global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(const ProductArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bars[3 * kMaxStages + 4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_word;
+  __shared__ double sums[kProductThreads / 32];
+  __shared__ int last;
+  const uint32_t raw = ptx::smem_u32(smem_raw);
+  const uint32_t base = (raw + 1023u) & ~1023u;
+  uint8_t* gen = smem_raw + (base - raw);
+  volatile int* abort_flag = &abort_word;
+  const int widest = a.padded < kChunk ? a.padded : kChunk;
+  const uint32_t b_bytes = static_cast<uint32_t>(widest) * 128u;
+  const uint32_t stage_bytes = 2u * kPieceBytes + 2u * b_bytes;
+  const uint32_t bar0 = ptx::smem_u32(bars);
+  auto ready_bar = [&](int s) { return bar0 + s * 8; };                   // the probabilities' pieces
+  auto full_bar = [&](int s) { return bar0 + (kMaxStages + s) * 8; };     // the counts' pieces
+  auto empty_bar = [&](int s) { return bar0 + (2 * kMaxStages + s) * 8; };
+  auto tfull_bar = [&](int i) { return bar0 + (3 * kMaxStages + i) * 8; };
+  auto tempty_bar = [&](int i) { return bar0 + (3 * kMaxStages + 2 + i) * 8; };
+  const int warp = __shfl_sync(kFull, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+  const int blocks = a.padded / 64;
+
+  if (warp == 0 && ptx::elect_one()) {
+    for (int s = 0; s < a.stages; ++s) {
+      ptx::mbar_init(ready_bar(s), kMakers);
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(tfull_bar(i), 1);
+      ptx::mbar_init(tempty_bar(i), 4);
+    }
+    abort_word = 0;
+    ptx::mbar_fence_init();
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc(ptx::smem_u32(&tmem_slot), 512);
+    ptx::tmem_relinquish();
+  }
+  pdl_wait();
+  ptx::tc_fence_before();
   __syncthreads();
-  if (threadIdx.x == 0) {
-    for (int i = 1; i < 8; ++i) v += sums[i];
-    *loss = static_cast<float>(head->coef * (v + static_cast<double>(head->mean) * head->tokens));
-  }
-}
+  ptx::tc_fence_after();
+  const uint32_t tmem = tmem_slot;
+  const bool second = a.head->second != 0;
+  struct Item {
+    int64_t t0;
+    int h, chunk, n0, columns;
+  };
+  auto item_of = [&](int i) {
+    Item it;
+    it.h = BACKWARD ? i & 1 : 0;
+    const int j = BACKWARD ? i >> 1 : i;
+    it.chunk = j % a.chunks;
+    it.t0 = static_cast<int64_t>(j / a.chunks) * kTileTokens;
+    it.n0 = it.chunk * kChunk;
+    it.columns = a.padded - it.n0 < kChunk ? a.padded - it.n0 : kChunk;
+    return it;
+  };
 
-template <typename T>
-__global__ void __launch_bounds__(256) balance_backward_kernel(const T* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok,
-                                                               int nk, const Prepared* head, const float* c0, const float* c1,
-                                                               const float* token_s, const float* upstream, T* dlogits) {
-  extern __shared__ float p[];
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  softmax_tile<T>(logits, ts, hs, mask, t0, ntok, nk, p);
-  const float scale = static_cast<float>(head->coef * static_cast<double>(*upstream));
-  for (int h = 0; h < 2; ++h)
-    for (int i = threadIdx.x; i < nk; i += 256) {
-      float g[kTile];
-      product(h == 0 ? c0 : c1, p + (1 - h) * kTile * nk, nk, i, g);
-      for (int t = 0; t < kTile; ++t) {
-        if (t0 + t >= ntok) break;
-        const bool live = mask == nullptr || mask[t0 + t] != 0;
-        dlogits[((t0 + t) * 2 + h) * nk + i] =
-            from_f32<T>(live ? p[(h * kTile + t) * nk + i] * (g[t] - token_s[t0 + t]) * scale : 0.f);
+  // whole warps wait, and give up together
+  auto wait = [&](uint32_t bar, uint32_t parity) { return __all_sync(kFull, ptx::mbar_wait_bounded(bar, parity, abort_flag)) != 0; };
+
+  if (warp == 0) {
+    bool ok = true;
+    uint32_t use = 0;  // stages used so far
+    for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x) {
+      const Item it = item_of(i);
+      const int64_t per = static_cast<int64_t>(a.padded) * a.padded / 8;
+      const uint32_t bytes = static_cast<uint32_t>(it.columns) * 128u;
+      for (int kb = 0; kb < blocks; ++kb, ++use) {
+        const int s = use % a.stages;
+        ok = wait(empty_bar(s), ((use / a.stages) & 1u) ^ 1u);
+        if (!ok) break;
+        if (ptx::elect_one()) {
+          const uint4* src = a.pieces + 2 * it.h * per + (static_cast<int64_t>(kb) * a.padded + it.n0) * 8;
+          const uint32_t dst = base + s * stage_bytes + 2 * kPieceBytes;
+          ptx::mbar_arrive_expect_tx(full_bar(s), second ? 2 * bytes : bytes);
+          bulk_copy(dst, src, bytes, full_bar(s));
+          if (second) bulk_copy(dst + b_bytes, src + per, bytes, full_bar(s));
+        }
+        __syncwarp();
       }
     }
-}
-
-size_t matrix_bytes(int nk) { return align_up(static_cast<size_t>(nk) * nk * sizeof(float), 256); }
-constexpr int kMaxKeys = 2048;
-
-template <typename T>
-int forward_typed(const void* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok, int nk, const float* c0,
-                  const Prepared* head, float* token_s, double* part, float* loss, cudaStream_t stream) {
-  const int64_t tiles = (ntok + kTile - 1) / kTile;
-  const int smem = 2 * kTile * nk * 4;
-  if (tiles > 0) {
-    FMOE_CUDA_TRY(allow_smem(balance_forward_kernel<T>, smem));
-    balance_forward_kernel<T><<<static_cast<unsigned>(tiles), 256, smem, stream>>>(static_cast<const T*>(logits), ts, hs, mask, ntok, nk, c0, token_s, part);
-    FMOE_LAUNCH_CHECK();
+    if (!ok) {  // let the copies already requested land before the CTA goes away (bounded)
+      const uint32_t first = use > static_cast<uint32_t>(a.stages) ? use - a.stages : 0;
+      for (uint32_t u = first; u < use; ++u) ptx::mbar_wait_drain(full_bar(u % a.stages), (u / a.stages) & 1u);
+    }
+  } else if (warp == 1) {
+    bool ok = true;
+    uint32_t use = 0, round = 0;
+    for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x, ++round) {
+      const Item it = item_of(i);
+      const uint32_t acc = round & 1u;
+      ok = wait(tempty_bar(acc), ((round >> 1) & 1u) ^ 1u);
+      // float16 operands, float32 accumulator, 128 rows
+      const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(it.columns >> 3) << 17) | (8u << 24);
+      for (int kb = 0; kb < blocks && ok; ++kb, ++use) {
+        const int s = use % a.stages;
+        ok = wait(full_bar(s), (use / a.stages) & 1u) && wait(ready_bar(s), (use / a.stages) & 1u);
+        if (!ok) break;
+        ptx::tc_fence_after();
+        const uint32_t st = base + s * stage_bytes;
+        const uint64_t hi = ptx::umma_desc_kmajor_sw128(st), lo = ptx::umma_desc_kmajor_sw128(st + kPieceBytes);
+        const uint64_t c_hi = ptx::umma_desc_kmajor_sw128(st + 2 * kPieceBytes);
+        const uint64_t c_lo = ptx::umma_desc_kmajor_sw128(st + 2 * kPieceBytes + b_bytes);
+        if (ptx::elect_one()) {
+          const uint32_t d = tmem + acc * kChunk;
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) {
+            ptx::umma_bf16_ss(d, hi + 2 * kk, c_hi + 2 * kk, idesc, (kb | kk) != 0 ? 1u : 0u);
+            ptx::umma_bf16_ss(d, lo + 2 * kk, c_hi + 2 * kk, idesc, 1u);
+            if (second) ptx::umma_bf16_ss(d, hi + 2 * kk, c_lo + 2 * kk, idesc, 1u);
+          }
+          ptx::umma_commit(empty_bar(s));
+          if (kb == blocks - 1) ptx::umma_commit(tfull_bar(acc));
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp < 6) {
+    bool ok = true;
+    uint32_t round = 0;
+    const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
+    const float unscale = a.head->unscale;
+    const float scale = BACKWARD ? static_cast<float>(a.head->coef * static_cast<double>(*a.upstream)) : 0.f;
+    for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x, ++round) {
+      const Item it = item_of(i);
+      const uint32_t acc = round & 1u;
+      const int64_t t = it.t0 + quarter * 32 + lane;
+      float top = 0.f, inv = 0.f, s = 0.f;
+      if (t < a.ntok) {
+        const float4 st = a.stats[t];
+        top = it.h == 0 ? st.x : st.z;
+        inv = it.h == 0 ? st.y : st.w;
+        if (BACKWARD)
+          for (int c = 0; c < a.chunks; ++c) s += a.token_s[static_cast<int64_t>(c) * a.ntok + t];
+      }
+      const bool live = inv != 0.f;
+      const T* row = static_cast<const T*>(a.logits) + t * a.ts + it.h * a.hs;
+      T* out = BACKWARD ? static_cast<T*>(a.dlogits) + (t * 2 + it.h) * a.nk : nullptr;
+      ok = wait(tfull_bar(acc), (round >> 1) & 1u);
+      if (!ok) break;
+      ptx::tc_fence_after();
+      const uint32_t taddr = tmem + acc * kChunk + (static_cast<uint32_t>(quarter * 32) << 16);
+      for (int c = 0; c < it.columns; c += 32) {
+        float x[4][8];
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[v][k] = 0.f;
+          if (live) load_logits<T, VEC>(row, it.n0 + c + v * 8, a.nk, x[v]);
+        }
+        uint32_t r[32];
+        ptx::tmem_ld_32x32(taddr + c, r);
+        ptx::tmem_ld_wait(r);
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int col = it.n0 + c + v * 8;
+          float o[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float p = live && col + k < a.nk ? probability(x[v][k], top, inv) : 0.f;
+            const float g = __uint_as_float(r[v * 8 + k]);
+            if (BACKWARD) o[k] = live ? p * fmaf(g, unscale, -s) * scale : 0.f;
+            else if (live && col + k < a.nk) s = fmaf(p, g, s);
+          }
+          if (BACKWARD && t < a.ntok) {
+            if (VEC) {
+#pragma unroll
+              for (int k = 0; k < 8; k += Vec16<T>::N)
+                if (col + k < a.nk) *reinterpret_cast<uint4*>(out + col + k) = pack16<T>(*reinterpret_cast<float (*)[Vec16<T>::N]>(&o[k]));
+            } else {
+#pragma unroll
+              for (int k = 0; k < 8; ++k)
+                if (col + k < a.nk) out[col + k] = from_f32<T>(o[k]);
+            }
+          }
+        }
+      }
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(tempty_bar(acc));
+      if (!BACKWARD) {
+        s *= unscale;
+        if (t < a.ntok) a.token_s[static_cast<int64_t>(it.chunk) * a.ntok + t] = s;
+        double all = s;
+        for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(kFull, all, d);
+        if (lane == 0) a.part[static_cast<int64_t>(i) * 4 + quarter] = all;
+      }
+    }
+  } else {
+    bool ok = true;
+    uint32_t use = 0;
+    // thread -> rows r0, r0 + 32, ... and a fixed 16-byte place (8 columns) of each 64-column block
+    const int id = threadIdx.x - 6 * 32, piece = id & 7, r0 = id >> 3;
+    const int place = piece ^ (r0 & 7);
+    constexpr int kRows = kTileTokens / (kMakers * 4);
+    for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x) {
+      const Item it = item_of(i);
+      const T* rows[kRows];
+      float top[kRows], inv[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const int64_t t = it.t0 + r0 + r * (kMakers * 4);
+        top[r] = inv[r] = 0.f;
+        rows[r] = static_cast<const T*>(a.logits) + t * a.ts + (1 - it.h) * a.hs;
+        if (t < a.ntok) {
+          const float4 st = a.stats[t];
+          top[r] = it.h == 0 ? st.z : st.x;
+          inv[r] = it.h == 0 ? st.w : st.y;
+        }
+      }
+      for (int kb = 0; kb < blocks; ++kb, ++use) {
+        const int s = use % a.stages;
+        const int col = kb * 64 + piece * 8;
+        float x[kRows][8];
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+          for (int k = 0; k < 8; ++k) x[r][k] = 0.f;
+          if (inv[r] != 0.f) load_logits<T, VEC>(rows[r], col, a.nk, x[r]);
+        }
+        ok = wait(empty_bar(s), ((use / a.stages) & 1u) ^ 1u);
+        if (!ok) break;
+        uint4* dst = reinterpret_cast<uint4*>(gen + s * stage_bytes);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          float hi[8], lo[8];
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const float p = inv[r] != 0.f && col + k < a.nk ? probability(x[r][k], top[r], inv[r]) * 32768.f : 0.f;
+            hi[k] = round_to<__half>(p);
+            lo[k] = p - hi[k];
+          }
+          const int at = (r0 + r * (kMakers * 4)) * 8 + place;
+          dst[at] = pack16<__half>(hi);
+          dst[at + kPieceBytes / 16] = pack16<__half>(lo);
+        }
+        ptx::fence_async_smem();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(ready_bar(s));
+      }
+    }
   }
-  balance_loss_kernel<<<1, 256, 0, stream>>>(head, part, tiles, loss);
-  FMOE_LAUNCH_CHECK();
-  return FMOE_OK;
+
+  __syncwarp();
+  ptx::tc_fence_before();
+  __threadfence();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+  if (threadIdx.x == 0 && abort_word != 0 && a.status != nullptr) atomicOr(a.status, FMOE_STATUS_WAIT_TIMEOUT);
+  if (BACKWARD) return;
+  // the CTA that ends last adds the items' sums, in their order
+  if (threadIdx.x == 0) last = atomicAdd(a.finished, 1u) == gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  double v = 0.0;
+  for (int i = threadIdx.x; i < 4 * a.items; i += kProductThreads) v += static_cast<const volatile double*>(a.part)[i];
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
+  if (lane == 0) sums[warp] = v;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int i = 1; i < kProductThreads / 32; ++i) v += sums[i];
+    *a.loss = static_cast<float>(a.head->coef * (v + static_cast<double>(a.head->mean) * a.head->tokens));
+  }
+}
+
+size_t matrix_bytes(int nk) { return static_cast<size_t>(padded_keys(nk)) * padded_keys(nk) * 2; }
+int64_t token_tiles(int64_t T) { return (T + kTileTokens - 1) / kTileTokens; }
+
+template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStream_t stream) {
+  constexpr int V = Vec16<T>::N;
+  const bool vec = a.nk % V == 0 && a.ts % V == 0 && a.hs % V == 0 && aligned16(a.logits) && (!BACKWARD || aligned16(a.dlogits));
+  const int widest = a.padded < kChunk ? a.padded : kChunk;
+  const int stage = 2 * kPieceBytes + 2 * widest * 128;
+  a.stages = 200 * 1024 / stage;
+  if (a.stages > kMaxStages) a.stages = kMaxStages;
+  const int smem = a.stages * stage + 1024;
+  const int64_t items = token_tiles(a.ntok) * a.chunks * (BACKWARD ? 2 : 1);
+  if (items > 0x7FFFFFFF / 4) return FMOE_ERR_UNSUPPORTED;
+  a.items = static_cast<int>(items);
+  const int grid = a.items < device_sm_count() ? a.items : device_sm_count();
+  auto run = [&](auto* kern) -> int {
+    FMOE_CUDA_TRY(allow_smem(kern, smem));
+    FMOE_CUDA_TRY(launch_pdl(BACKWARD ? 0 : 32, kern, dim3(grid), dim3(kProductThreads), smem, stream, 1, a));
+    return FMOE_OK;
+  };
+  return vec ? run(balance_product_kernel<T, true, BACKWARD>) : run(balance_product_kernel<T, false, BACKWARD>);
 }
 
 template <typename T>
-int backward_typed(const void* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok, int nk, const Prepared* head,
-                   const float* c0, const float* c1, const float* token_s, const float* upstream, void* dlogits, cudaStream_t stream) {
-  const int64_t tiles = (ntok + kTile - 1) / kTile;
-  const int smem = 2 * kTile * nk * 4;
-  FMOE_CUDA_TRY(allow_smem(balance_backward_kernel<T>, smem));
-  balance_backward_kernel<T><<<static_cast<unsigned>(tiles), 256, smem, stream>>>(static_cast<const T*>(logits), ts, hs, mask, ntok, nk, head, c0, c1,
-                                                                                 token_s, upstream, static_cast<T*>(dlogits));
+int forward_typed(ProductArgs a, const uint8_t* mask, const int64_t* counts, Prepared* head, float4* stats, Part* part, cudaStream_t stream) {
+  const int64_t want = (a.ntok + 7) / 8, cap = static_cast<int64_t>(device_sm_count()) * 8;
+  const int64_t grid = want > cap ? cap : want < kParts ? kParts : want;
+  balance_stats_kernel<T><<<static_cast<unsigned>(grid), 256, 0, stream>>>(static_cast<const T*>(a.logits), a.ts, a.hs, mask, a.ntok, a.nk,
+                                                                          stats, counts, part);
   FMOE_LAUNCH_CHECK();
-  return FMOE_OK;
+  const int64_t pieces = static_cast<int64_t>(a.padded) * a.padded / 4;
+  FMOE_CUDA_TRY(launch_pdl(32, balance_prepare_kernel, dim3(static_cast<unsigned>((pieces + 255) / 256)), dim3(256), 0, stream, 1, counts,
+                           a.nk, a.padded, part, head, const_cast<uint4*>(a.pieces)));
+  return launch_product<T, false>(a, stream);
 }
 
 }  // namespace
@@ -228,50 +559,80 @@ int launch_expert_counts(const int64_t* indices, const uint8_t* mask, int64_t T,
   return FMOE_OK;
 }
 
-size_t balance_prepared_bytes(int nk) { return nk <= 0 || nk > kMaxKeys ? 0 : 256 + 2 * matrix_bytes(nk); }
-size_t balance_workspace_bytes(int64_t T) {
-  return T < 0 ? 0 : kParts * sizeof(Part) + static_cast<size_t>((T + kTile - 1) / kTile) * sizeof(double);
+size_t balance_prepared_bytes(int nk) { return nk <= 0 || nk > kMaxKeys ? 0 : kHeadBytes + 4 * matrix_bytes(nk); }
+size_t balance_stats_floats(int64_t T, int nk) { return T <= 0 || nk <= 0 || nk > kMaxKeys ? 0 : static_cast<size_t>(T) * (4 + column_chunks(nk)); }
+size_t balance_workspace_bytes(int64_t T, int nk) {
+  if (T < 0 || nk <= 0 || nk > kMaxKeys) return 0;
+  return kParts * sizeof(Part) + static_cast<size_t>(token_tiles(T)) * column_chunks(nk) * 4 * sizeof(double);
 }
 
 int launch_balance_forward(const void* logits, int64_t ts, int64_t hs, int dtype, const int64_t* counts, const uint8_t* mask, int64_t T,
-                           int nk, float* loss, float* token_s, void* prepared, size_t prepared_bytes, void* ws, size_t ws_bytes,
-                           cudaStream_t stream) {
+                           int nk, float* loss, float* stats, void* prepared, size_t prepared_bytes, void* ws, size_t ws_bytes,
+                           int32_t* status, cudaStream_t stream) {
   if (T < 0 || nk <= 0 || counts == nullptr || loss == nullptr) return FMOE_ERR_BAD_ARG;
   if (nk > kMaxKeys) return FMOE_ERR_UNSUPPORTED;
-  if (T > 0 && (logits == nullptr || token_s == nullptr)) return FMOE_ERR_BAD_ARG;
-  if (prepared == nullptr || prepared_bytes < balance_prepared_bytes(nk) || ws == nullptr || ws_bytes < balance_workspace_bytes(T)) return FMOE_ERR_WORKSPACE;
+  if (T == 0) {
+    FMOE_CUDA_TRY(cudaMemsetAsync(loss, 0, sizeof(float), stream));
+    return FMOE_OK;
+  }
+  if (logits == nullptr || stats == nullptr) return FMOE_ERR_BAD_ARG;
+  if (prepared == nullptr || prepared_bytes < balance_prepared_bytes(nk) || ws == nullptr || ws_bytes < balance_workspace_bytes(T, nk)) return FMOE_ERR_WORKSPACE;
+  if (!aligned16(stats) || !aligned16(prepared) || !aligned16(ws)) return FMOE_ERR_ALIGNMENT;
   Prepared* head = static_cast<Prepared*>(prepared);
-  float* c0 = reinterpret_cast<float*>(static_cast<char*>(prepared) + 256);
-  float* c1 = reinterpret_cast<float*>(static_cast<char*>(prepared) + 256 + matrix_bytes(nk));
-  Part* sums = static_cast<Part*>(ws);
-  double* part = reinterpret_cast<double*>(sums + kParts);
-  balance_sums_kernel<<<kParts, 256, 0, stream>>>(counts, nk * nk, mask, T, sums);
-  FMOE_LAUNCH_CHECK();
-  balance_prepare_kernel<<<(nk * nk + 1023) / 1024, 256, 0, stream>>>(counts, nk, mask != nullptr, T, sums, head, c0, c1);
-  FMOE_LAUNCH_CHECK();
+  Part* part = static_cast<Part*>(ws);
+  ProductArgs a = {};
+  a.logits = logits;
+  a.ts = ts;
+  a.hs = hs;
+  a.ntok = T;
+  a.stats = reinterpret_cast<const float4*>(stats);
+  a.token_s = stats + 4 * T;
+  a.head = head;
+  a.pieces = reinterpret_cast<const uint4*>(static_cast<char*>(prepared) + kHeadBytes);
+  a.part = reinterpret_cast<double*>(part + kParts);
+  a.loss = loss;
+  a.finished = &head->finished;
+  a.status = status;
+  a.nk = nk;
+  a.padded = padded_keys(nk);
+  a.chunks = column_chunks(nk);
+  float4* st = reinterpret_cast<float4*>(stats);
   switch (dtype) {
-    case FMOE_DTYPE_F32: return forward_typed<float>(logits, ts, hs, mask, T, nk, c0, head, token_s, part, loss, stream);
-    case FMOE_DTYPE_BF16: return forward_typed<__nv_bfloat16>(logits, ts, hs, mask, T, nk, c0, head, token_s, part, loss, stream);
-    case FMOE_DTYPE_F16: return forward_typed<__half>(logits, ts, hs, mask, T, nk, c0, head, token_s, part, loss, stream);
+    case FMOE_DTYPE_F32: return forward_typed<float>(a, mask, counts, head, st, part, stream);
+    case FMOE_DTYPE_BF16: return forward_typed<__nv_bfloat16>(a, mask, counts, head, st, part, stream);
+    case FMOE_DTYPE_F16: return forward_typed<__half>(a, mask, counts, head, st, part, stream);
     default: return FMOE_ERR_BAD_ARG;
   }
 }
 
-int launch_balance_backward(const void* logits, int64_t ts, int64_t hs, int dtype, const uint8_t* mask, int64_t T, int nk,
-                            const float* token_s, const void* prepared, size_t prepared_bytes, const float* upstream, void* dlogits,
+int launch_balance_backward(const void* logits, int64_t ts, int64_t hs, int dtype, int64_t T, int nk, const float* stats,
+                            const void* prepared, size_t prepared_bytes, const float* upstream, void* dlogits, int32_t* status,
                             cudaStream_t stream) {
   if (T < 0 || nk <= 0) return FMOE_ERR_BAD_ARG;
   if (nk > kMaxKeys) return FMOE_ERR_UNSUPPORTED;
   if (T == 0) return FMOE_OK;
-  if (logits == nullptr || token_s == nullptr || upstream == nullptr || dlogits == nullptr) return FMOE_ERR_BAD_ARG;
+  if (logits == nullptr || stats == nullptr || upstream == nullptr || dlogits == nullptr) return FMOE_ERR_BAD_ARG;
   if (prepared == nullptr || prepared_bytes < balance_prepared_bytes(nk)) return FMOE_ERR_WORKSPACE;
-  const Prepared* head = static_cast<const Prepared*>(prepared);
-  const float* c0 = reinterpret_cast<const float*>(static_cast<const char*>(prepared) + 256);
-  const float* c1 = reinterpret_cast<const float*>(static_cast<const char*>(prepared) + 256 + matrix_bytes(nk));
+  if (!aligned16(stats) || !aligned16(prepared)) return FMOE_ERR_ALIGNMENT;
+  ProductArgs a = {};
+  a.logits = logits;
+  a.ts = ts;
+  a.hs = hs;
+  a.ntok = T;
+  a.stats = reinterpret_cast<const float4*>(stats);
+  a.token_s = const_cast<float*>(stats) + 4 * T;
+  a.head = static_cast<const Prepared*>(prepared);
+  a.pieces = reinterpret_cast<const uint4*>(static_cast<const char*>(prepared) + kHeadBytes);
+  a.upstream = upstream;
+  a.dlogits = dlogits;
+  a.status = status;
+  a.nk = nk;
+  a.padded = padded_keys(nk);
+  a.chunks = column_chunks(nk);
   switch (dtype) {
-    case FMOE_DTYPE_F32: return backward_typed<float>(logits, ts, hs, mask, T, nk, head, c0, c1, token_s, upstream, dlogits, stream);
-    case FMOE_DTYPE_BF16: return backward_typed<__nv_bfloat16>(logits, ts, hs, mask, T, nk, head, c0, c1, token_s, upstream, dlogits, stream);
-    case FMOE_DTYPE_F16: return backward_typed<__half>(logits, ts, hs, mask, T, nk, head, c0, c1, token_s, upstream, dlogits, stream);
+    case FMOE_DTYPE_F32: return launch_product<float, true>(a, stream);
+    case FMOE_DTYPE_BF16: return launch_product<__nv_bfloat16, true>(a, stream);
+    case FMOE_DTYPE_F16: return launch_product<__half, true>(a, stream);
     default: return FMOE_ERR_BAD_ARG;
   }
 }

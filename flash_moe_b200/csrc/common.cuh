@@ -62,8 +62,8 @@ template <typename K> inline cudaError_t resident_ctas(K* kern, int threads, int
 // measured: the scores pass (4) is slower when it is made resident early - at the benchmark shape 215 vs 213 us per
 // step, at 131072 tokens x 2048 columns 15.4 vs 13.4 ms per layer - so it keeps the plain stream order; the other four
 // together give 211 vs 213 us in a graph and 214 vs 224 us launched eagerly
-constexpr int kPdlDefaultMask = 27;
-bool pdl_enabled(int kernel_class);  // api.cu; classes: 1 router GEMM, 2 top-k, 4 scores, 8 accumulate, 16 MLP GEMMs
+constexpr int kPdlDefaultMask = 59;
+bool pdl_enabled(int kernel_class);  // api.cu; classes: 1 router GEMM, 2 top-k, 4 scores, 8 accumulate, 16 MLP GEMMs, 32 balance loss
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // What the kernel before this one may write is read behind pdl_wait() through pointers without __restrict__, by ordinary or
@@ -311,12 +311,13 @@ int launch_grad_norm(void* const* grads, const int64_t* numels, const int32_t* d
 int launch_expert_counts(const int64_t* indices, const uint8_t* mask, int64_t T, int k, int64_t N, int64_t* counts, int32_t* status,
                          cudaStream_t stream);
 size_t balance_prepared_bytes(int nk);
-size_t balance_workspace_bytes(int64_t T);
+size_t balance_stats_floats(int64_t T, int nk);
+size_t balance_workspace_bytes(int64_t T, int nk);
 int launch_balance_forward(const void* logits, int64_t ts, int64_t hs, int dtype, const int64_t* counts, const uint8_t* mask, int64_t T,
-                           int nk, float* loss, float* token_s, void* prepared, size_t prepared_bytes, void* ws, size_t ws_bytes,
-                           cudaStream_t stream);
-int launch_balance_backward(const void* logits, int64_t ts, int64_t hs, int dtype, const uint8_t* mask, int64_t T, int nk,
-                            const float* token_s, const void* prepared, size_t prepared_bytes, const float* upstream, void* dlogits,
+                           int nk, float* loss, float* stats, void* prepared, size_t prepared_bytes, void* ws, size_t ws_bytes,
+                           int32_t* status, cudaStream_t stream);
+int launch_balance_backward(const void* logits, int64_t ts, int64_t hs, int dtype, int64_t T, int nk, const float* stats,
+                            const void* prepared, size_t prepared_bytes, const float* upstream, void* dlogits, int32_t* status,
                             cudaStream_t stream);
 int launch_combine_rows(const float* rows, int64_t num_rows, const int32_t* slot, int num_sources, int64_t ntok, int H,
                         float* out, int32_t* status, cudaStream_t stream);

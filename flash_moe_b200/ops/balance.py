@@ -59,25 +59,26 @@ def _loss_forward(logits, counts, mask):
     L = _lib.lib()
     logits, ts, hs = _strided(logits)
     loss = torch.empty((), dtype=torch.float32, device=dev)
-    stats = torch.empty(T, dtype=torch.float32, device=dev)
+    stats = torch.empty(L.fmoe_balance_loss_stats_floats(T, nk), dtype=torch.float32, device=dev)
     prepared = torch.empty(L.fmoe_balance_loss_prepared_bytes(nk), dtype=torch.uint8, device=dev)
-    ws = torch.empty(L.fmoe_balance_loss_workspace_bytes(T), dtype=torch.uint8, device=dev)
+    ws = torch.empty(L.fmoe_balance_loss_workspace_bytes(T, nk), dtype=torch.uint8, device=dev)
     rc = _lib.call("fmoe_balance_loss_forward", dev, logits.data_ptr(), ts, hs, _lib.dtype_code(logits), counts.data_ptr(),
                    _lib.ptr(mask), T, nk, loss.data_ptr(), stats.data_ptr(), prepared.data_ptr(), prepared.numel(), ws.data_ptr(),
-                   ws.numel())
+                   ws.numel(), _lib.status_ptr(dev))
     if rc:
         _lib.check(rc, "fmoe_balance_loss_forward")
     return loss, stats, prepared
 
 
-def _loss_backward(logits, mask, stats, prepared, upstream):
+def _loss_backward(logits, stats, prepared, upstream):
     dev = logits.device
     _, T, nk = logits.shape
     logits, ts, hs = _strided(logits)
     # the rows of both halves of a token next to each other, as the router's product writes its logits
     dlogits = torch.empty((T, 2, nk), dtype=logits.dtype, device=dev)
-    rc = _lib.call("fmoe_balance_loss_backward", dev, logits.data_ptr(), ts, hs, _lib.dtype_code(logits), _lib.ptr(mask), T, nk,
-                   stats.data_ptr(), prepared.data_ptr(), prepared.numel(), upstream.data_ptr(), dlogits.data_ptr())
+    rc = _lib.call("fmoe_balance_loss_backward", dev, logits.data_ptr(), ts, hs, _lib.dtype_code(logits), T, nk,
+                   stats.data_ptr(), prepared.data_ptr(), prepared.numel(), upstream.data_ptr(), dlogits.data_ptr(),
+                   _lib.status_ptr(dev))
     if rc:
         _lib.check(rc, "fmoe_balance_loss_backward")
     return dlogits.transpose(0, 1)
@@ -87,17 +88,17 @@ class BalanceLossFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, router_logits, counts, mask):
         loss, stats, prepared = _loss_forward(router_logits, counts, mask)
-        ctx.save_for_backward(router_logits, mask, stats, prepared)
+        ctx.save_for_backward(router_logits, stats, prepared)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, upstream):
-        logits, mask, stats, prepared = ctx.saved_tensors
+        logits, stats, prepared = ctx.saved_tensors
         if not ctx.needs_input_grad[0]:
             return None, None, None
         upstream = upstream.to(torch.float32).contiguous()
-        return _loss_backward(logits, contiguous(mask), contiguous(stats), contiguous(prepared), upstream), None, None
+        return _loss_backward(logits, contiguous(stats), contiguous(prepared), upstream), None, None
 
 
 def balance_loss(router_logits: torch.Tensor, counts: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:

@@ -251,17 +251,19 @@ int fmoe_expert_counts(const int64_t* indices, const uint8_t* token_mask, int64_
  *   *loss = num_keys^2 sum_ij (C_ij / sum C) mean_t p_0[t,i] p_1[t,j],  the mean over the tokens of token_mask (nullable: all);
  *   dlogits [T, 2, num_keys] = its gradient times *upstream (one float in device memory), rows of masked tokens zero.
  * The loss is 0, and so is its gradient, where there is no selection or no token.  Value i of token t and half h of the logits is at
- * logits[t * token_stride + h * half_stride + i].  The forward leaves token_stats [T] and `prepared` for the backward.
+ * logits[t * token_stride + h * half_stride + i].  The forward leaves token_stats (fmoe_balance_loss_stats_floats floats) and
+ * `prepared` for the backward; both and the workspace are 16-byte aligned.  num_keys is at most 2048.
  */
 size_t fmoe_balance_loss_prepared_bytes(int num_keys);
-size_t fmoe_balance_loss_workspace_bytes(int64_t num_tokens);
+size_t fmoe_balance_loss_stats_floats(int64_t num_tokens, int num_keys);
+size_t fmoe_balance_loss_workspace_bytes(int64_t num_tokens, int num_keys);
 int fmoe_balance_loss_forward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, const int64_t* counts,
                               const uint8_t* token_mask, int64_t num_tokens, int num_keys, float* loss, float* token_stats,
-                              void* prepared, size_t prepared_bytes, void* workspace, size_t workspace_bytes,
+                              void* prepared, size_t prepared_bytes, void* workspace, size_t workspace_bytes, int32_t* status,
                               fmoe_stream_t stream);
-int fmoe_balance_loss_backward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, const uint8_t* token_mask,
-                               int64_t num_tokens, int num_keys, const float* token_stats, const void* prepared,
-                               size_t prepared_bytes, const float* upstream, void* dlogits, fmoe_stream_t stream);
+int fmoe_balance_loss_backward(const void* logits, int64_t token_stride, int64_t half_stride, int dtype, int64_t num_tokens,
+                               int num_keys, const float* token_stats, const void* prepared, size_t prepared_bytes,
+                               const float* upstream, void* dlogits, int32_t* status, fmoe_stream_t stream);
 
 /*
  * Self-test of the bounded device-side waits (no counterpart in the reference): a one-thread kernel waits on a

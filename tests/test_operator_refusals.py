@@ -54,12 +54,12 @@ def test_counts(lib):
 
 
 def test_loss(lib):
-    prepared, ws = lib.fmoe_balance_loss_prepared_bytes(8), lib.fmoe_balance_loss_workspace_bytes(4)
+    prepared, ws = lib.fmoe_balance_loss_prepared_bytes(8), lib.fmoe_balance_loss_workspace_bytes(4, 8)
     assert prepared > 0 and ws > 0
     assert lib.fmoe_balance_loss_prepared_bytes(0) == 0 and lib.fmoe_balance_loss_prepared_bytes(2049) == 0
 
     def forward(logits=p(), dtype=1, counts=p(2), T=4, nk=8, loss=p(3), stats=p(4), prep=p(5), prep_bytes=prepared, w=p(6), w_bytes=ws):
-        return lib.fmoe_balance_loss_forward(logits, 16, 8, dtype, counts, None, T, nk, loss, stats, prep, prep_bytes, w, w_bytes, None)
+        return lib.fmoe_balance_loss_forward(logits, 16, 8, dtype, counts, None, T, nk, loss, stats, prep, prep_bytes, w, w_bytes, None, None)
 
     assert forward(logits=None) == BAD_ARG and forward(counts=None) == BAD_ARG and forward(loss=None) == BAD_ARG
     assert forward(stats=None) == BAD_ARG and forward(T=-1) == BAD_ARG and forward(nk=0) == BAD_ARG and forward(dtype=9) == BAD_ARG
@@ -68,7 +68,7 @@ def test_loss(lib):
     assert forward(w=None) == WORKSPACE and forward(w_bytes=ws - 1) == WORKSPACE
 
     def backward(logits=p(), dtype=1, T=4, nk=8, stats=p(2), prep=p(3), prep_bytes=prepared, up=p(4), out=p(5)):
-        return lib.fmoe_balance_loss_backward(logits, 16, 8, dtype, None, T, nk, stats, prep, prep_bytes, up, out, None)
+        return lib.fmoe_balance_loss_backward(logits, 16, 8, dtype, T, nk, stats, prep, prep_bytes, up, out, None, None)
 
     assert backward(T=0) == OK
     for name in ("logits", "stats", "up", "out"):
@@ -135,7 +135,7 @@ def ops_without_a_gpu(monkeypatch):
     monkeypatch.setattr(norm, "_backward", lambda dn, ds, s, w, eps, want: (2 * dn if ds is None else 2 * dn + ds, torch.ones(s.shape[-1]) if want else None))
     monkeypatch.setattr(bal._lib, "require_cuda", lambda *t: t[0].device)
     monkeypatch.setattr(bal, "_loss_forward", lambda x, c, m: (torch.tensor(float(x.detach().sum())), torch.zeros(1), torch.zeros(1)))
-    monkeypatch.setattr(bal, "_loss_backward", lambda x, m, s, pr, up: up * torch.ones_like(x))
+    monkeypatch.setattr(bal, "_loss_backward", lambda x, s, pr, up: up * torch.ones_like(x))
 
 
 NORM = lambda x: add_rms_norm(x, x, None)[0]  # noqa: E731
