@@ -23,24 +23,77 @@ namespace {
 
 constexpr unsigned kFull = 0xFFFFFFFFu;
 
-__global__ void __launch_bounds__(256) expert_counts_kernel(const int64_t* indices, const uint8_t* mask, int64_t pairs, int k,
-                                                            int64_t N, unsigned long long* counts, int32_t* status) {
-  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < pairs; i += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t e = indices[i];
-    if (mask != nullptr && mask[i / k] == 0) continue;
-    if (e >= 0 && e < N) atomicAdd(counts + e, 1ull);
-    else if (e != -1 && status != nullptr) atomicOr(status, FMOE_STATUS_BAD_EXPERT_ID);
+// ------------------------------------------------------------------------------------------------ counts
+// Popular experts are selected again and again: at a Zipf exponent of 1.1 one id of a million takes an eighth of the selections,
+// and additions to one address follow one another (56 us for 524288 selections, all by global atomics).  So each CTA adds in
+// a small table in shared memory first, an id in one of two places of its own; an id that finds both taken by others goes to
+// global memory, and at the end so does each place of the table.  Whole numbers: the order changes nothing.
+constexpr int kCountThreads = 512;
+constexpr int kCountPlaces = 4096;
+
+__device__ __forceinline__ void count_one(int64_t e, int64_t N, int* ids, unsigned* seen, unsigned long long* counts, int32_t* status) {
+  if (e < 0 || e >= N) {
+    if (e != -1 && status != nullptr) atomicOr(status, FMOE_STATUS_BAD_EXPERT_ID);
+    return;
   }
+  if (e < 0x7FFFFFFF) {
+    const int id = static_cast<int>(e);
+    const unsigned place = (static_cast<unsigned>(id) * 2654435761u) >> 20;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const unsigned at = place ^ i;
+      int owner = *static_cast<volatile int*>(ids + at);
+      if (owner == -1) owner = atomicCAS(ids + at, -1, id);
+      if (owner == -1 || owner == id) {
+        atomicAdd(seen + at, 1u);
+        return;
+      }
+    }
+  }
+  atomicAdd(counts + e, 1ull);
+}
+
+// One cluster of CTAs clears the counts itself where the call is small: a launch less.
+template <bool CLEAR>
+__global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const int64_t* indices, const uint8_t* mask, int64_t pairs, int k,
+                                                                      int64_t N, unsigned long long* counts, int32_t* status) {
+  __shared__ int ids[kCountPlaces];
+  __shared__ unsigned seen[kCountPlaces];
+  const int64_t first = static_cast<int64_t>(blockIdx.x) * kCountThreads + threadIdx.x, step = static_cast<int64_t>(gridDim.x) * kCountThreads;
+  for (int i = threadIdx.x; i < kCountPlaces; i += kCountThreads) {
+    ids[i] = -1;
+    seen[i] = 0;
+  }
+  if (CLEAR) {
+    for (int64_t i = first; i < N; i += step) counts[i] = 0;
+    ptx::cluster_sync();
+  } else {
+    __syncthreads();
+  }
+  constexpr int kAhead = 4;
+  for (int64_t i0 = first; i0 < pairs; i0 += kAhead * step) {
+    int64_t e[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int64_t i = i0 + u * step;
+      e[u] = -1;
+      if (i < pairs && (mask == nullptr || mask[pairs <= 0xFFFFFFFFll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(k) : i / k] != 0)) e[u] = indices[i];
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) count_one(e[u], N, ids, seen, counts, status);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kCountPlaces; i += kCountThreads)
+    if (seen[i] != 0) atomicAdd(counts + ids[i], static_cast<unsigned long long>(seen[i]));
 }
 
 // ------------------------------------------------------------------------------------------------ statistics and counts
 constexpr int kParts = 64;  // CTAs that sum the counts
 constexpr int kMaxKeys = 2048;
 constexpr int kTileTokens = 128;
-constexpr int kChunk = 256;  // columns of a product that one CTA accumulates
+constexpr int kChunk = 256;  // columns of a product that one CTA accumulates, at most
 
 inline int padded_keys(int nk) { return (nk + 63) / 64 * 64; }
-inline int column_chunks(int nk) { return (padded_keys(nk) + kChunk - 1) / kChunk; }
 
 struct Part {
   double sum;
@@ -58,8 +111,53 @@ struct Prepared {
 };
 constexpr size_t kHeadBytes = 256;
 
+// exp(t) for t <= 0 by the exponential of base 2: within a few 2^-23 of it, values below 2^-126 become 0
+__device__ __forceinline__ float exp_below(float t) {
+  float v;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(t * 1.44269504f));
+  return v;
+}
+
+template <typename T> __device__ __forceinline__ uint32_t minus_infinity() { return 0xFF800000u; }
+template <> __device__ __forceinline__ uint32_t minus_infinity<__nv_bfloat16>() { return 0xFF80FF80u; }
+template <> __device__ __forceinline__ uint32_t minus_infinity<__half>() { return 0xFC00FC00u; }
+
+// Eight logits of a row from column c on, as they are loaded.  What lies behind the row's end, or in a row that is not read, is
+// minus infinity: its exponential is 0 and no use of the values has to ask.
+template <typename T, bool VEC> struct Logits;
+template <typename T> struct Logits<T, true> {  // rows made of aligned 16-byte pieces
+  static constexpr int kLoads = 8 / Vec16<T>::N;
+  uint4 q[kLoads];
+  __device__ __forceinline__ void load(const T* row, int c, int nk, bool read = true) {
+    const uint32_t none = minus_infinity<T>();
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      q[i] = make_uint4(none, none, none, none);
+      if (read && c + i * Vec16<T>::N < nk) q[i] = ld16(row + c + i * Vec16<T>::N);
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) unpack16<T>(q[i], *reinterpret_cast<float (*)[Vec16<T>::N]>(&f[i * Vec16<T>::N]));
+  }
+};
+template <typename T> struct Logits<T, false> {
+  T v[8];
+  __device__ __forceinline__ void load(const T* row, int c, int nk, bool read = true) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = from_f32<T>(-INFINITY);
+      if (read && c + i < nk) v[i] = row[c + i];
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(v[i]);
+  }
+};
+
 // (maximum, 1 / sum of exp(x - maximum)) of each half; 0, 0 for masked tokens, which are not read: no sum has an inverse of 0
-template <typename T>
+template <typename T, bool VEC>
 __global__ void __launch_bounds__(256) balance_stats_kernel(const T* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok,
                                                             int nk, float4* stats, const int64_t* counts, Part* part) {
   pdl_launch_dependents();
@@ -98,22 +196,69 @@ __global__ void __launch_bounds__(256) balance_stats_kernel(const T* logits, int
       part[blockIdx.x] = {c, top, mask != nullptr ? m : blockIdx.x == 0 ? static_cast<long long>(ntok) : 0ll};
     }
   }
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * 8 + warp; t < ntok; t += static_cast<int64_t>(gridDim.x) * 8) {
-    float out[4] = {0.f, 0.f, 0.f, 0.f};
-    if (mask == nullptr || mask[t] != 0) {
+  // A warp takes kRows tokens at a time.  A lane holds eight values of each row and 256 columns; longer rows are read again for
+  // the sum.
+  constexpr int kRows = 2;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 8 * kRows;
+  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * kRows; t0 < ntok; t0 += step) {
+    Logits<T, VEC> x[kRows][2];
+    float top[2 * kRows], sum[2 * kRows];
+    bool live[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) live[r] = t0 + r < ntok && (mask == nullptr || mask[t0 + r] != 0);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) x[r][h].load(logits + (t0 + r) * ts + h * hs, lane * 8, nk, live[r]);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const T* src = logits + t * ts + h * hs;
-        float top = -INFINITY, sum = 0.f;
-        for (int i = lane; i < nk; i += 32) top = fmaxf(top, to_f32<T>(src[i]));
-        for (int d = 16; d > 0; d >>= 1) top = fmaxf(top, __shfl_xor_sync(kFull, top, d));
-        for (int i = lane; i < nk; i += 32) sum += expf(to_f32<T>(src[i]) - top);
-        for (int d = 16; d > 0; d >>= 1) sum += __shfl_xor_sync(kFull, sum, d);
-        out[2 * h] = top;
-        out[2 * h + 1] = 1.f / sum;
+        float f[8], m;
+        x[r][h].get(f);
+        m = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
+        if (live[r])
+          for (int c = (32 + lane) * 8; c < nk; c += 256) {
+            Logits<T, VEC> y;
+            y.load(logits + (t0 + r) * ts + h * hs, c, nk);
+            y.get(f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = fmaxf(m, f[i]);
+          }
+        top[2 * r + h] = m;
       }
-    }
-    if (lane == 0) stats[t] = make_float4(out[0], out[1], out[2], out[3]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < 2 * kRows; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(kFull, top[i], d));
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float f[8], v = 0.f;
+        const float m = top[2 * r + h];
+        x[r][h].get(f);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v += exp_below(f[i] - m);
+        if (live[r])
+          for (int c = (32 + lane) * 8; c < nk; c += 256) {
+            Logits<T, VEC> y;
+            y.load(logits + (t0 + r) * ts + h * hs, c, nk);
+            y.get(f);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v += exp_below(f[i] - m);
+          }
+        sum[2 * r + h] = v;
+      }
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+      for (int i = 0; i < 2 * kRows; ++i) sum[i] += __shfl_xor_sync(kFull, sum[i], d);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r)
+      if (lane == r && t0 + r < ntok)
+        stats[t0 + r] = live[r] ? make_float4(top[2 * r], 1.f / sum[2 * r], top[2 * r + 1], 1.f / sum[2 * r + 1])
+                                : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
@@ -124,12 +269,18 @@ __global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* cou
                                                               uint4* pieces) {
   pdl_launch_dependents();
   pdl_wait();
-  double sum = 0.0;
-  long long top = 0, tokens = 0;
-  for (int i = 0; i < kParts; ++i) {
-    sum += part[i].sum;
-    tokens += part[i].tokens;
-    top = part[i].top > top ? part[i].top : top;
+  // every warp adds the parts itself, in the same order
+  const int lane = threadIdx.x & 31;
+  static_assert(kParts == 64, "two parts a lane");
+  double sum = part[lane].sum + part[lane + 32].sum;
+  long long tokens = part[lane].tokens + part[lane + 32].tokens;
+  long long top = part[lane].top > part[lane + 32].top ? part[lane].top : part[lane + 32].top;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    sum += __shfl_xor_sync(kFull, sum, d);
+    tokens += __shfl_xor_sync(kFull, tokens, d);
+    const long long o = __shfl_xor_sync(kFull, top, d);
+    top = o > top ? o : top;
   }
   const double n = static_cast<double>(nk) * nk;
   const double mean = rint(sum / n);
@@ -145,7 +296,8 @@ __global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* cou
     head->second = second;
     head->finished = 0;
   }
-  const double scale = ldexp(1.0, -shift);
+  const long long taken = static_cast<long long>(mean);
+  const float scale = ldexpf(1.f, -shift);
   const int64_t per = static_cast<int64_t>(padded) * padded / 8;  // 16-byte pieces of one matrix
   const int64_t at = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
   if (at >= 2 * per) return;
@@ -166,9 +318,9 @@ __global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* cou
     float v = 0.f, rest = 0.f;
     if (row < nk && k < nk) {
       const long long c = h == 0 ? counts[static_cast<int64_t>(row) * nk + k] : counts[static_cast<int64_t>(k) * nk + row];
-      const double d = (static_cast<double>(c) - mean) * scale;
-      v = __half2float(__double2half(d));
-      rest = static_cast<float>(d - static_cast<double>(v));
+      const float d = static_cast<float>(c - taken) * scale;  // 24 bits, of which the two pieces keep 22
+      v = round_to<__half>(d);
+      rest = d - v;
     }
     hi[i] = v;
     lo[i] = rest;
@@ -183,11 +335,12 @@ __global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* cou
 // so that the second finds the logits in the L2 cache).  Warp roles, each a loop over the items of the CTA:
 //   0      copies the blocks of the counts' pieces into the ring
 //   1      issues the products of a stage: three of 128 x columns x 64, into one of two accumulators
-//   2..5   epilogue, a thread per token: probabilities p_h from the logits, with the accumulator's row
-//   6..13  make the stage's two pieces of p_(1-h), 128 x 64 each, from the logits
+//   2..9   epilogue, a thread per token and half of the columns: probabilities p_h from the logits, with the accumulator's row
+//   10..17 make the stage's two pieces of p_(1-h), 128 x 64 each, from the logits
+// Both kinds of readers of the logits have the next ones on the way while they work on the present ones.
 // Every wait is bounded; one that runs out raises FMOE_STATUS_WAIT_TIMEOUT and the CTA drains and leaves.
-constexpr int kMakers = 8;
-constexpr int kProductThreads = (6 + kMakers) * 32;
+constexpr int kMakers = 8, kReaders = 8;  // warps
+constexpr int kProductThreads = (2 + kReaders + kMakers) * 32;
 constexpr int kPieceBytes = kTileTokens * 128;  // one piece of the probabilities
 constexpr int kMaxStages = 4;
 
@@ -195,37 +348,19 @@ struct ProductArgs {
   const void* logits;
   int64_t ts, hs, ntok;
   const float4* stats;
-  float* token_s;  // [chunks][T]
+  float* token_s;  // [partial sums][T]
   const Prepared* head;
   const uint4* pieces;
-  double* part;           // forward: [items][4]
+  double* part;           // forward: [items][kReaders]
   float* loss;            // forward
   unsigned* finished;     // forward
   const float* upstream;  // backward
   void* dlogits;          // backward: [T, 2, nk]
   int32_t* status;
-  int nk, padded, chunks, stages;
-  int items;
+  int nk, padded, stages, items;
+  int width, chunks;  // columns of an item, items side by side
+  int partials;       // sums that make up s_t
 };
-
-// eight logits of a row from column c on; `whole`: an aligned piece inside the row
-template <typename T, bool VEC> __device__ __forceinline__ void load_logits(const T* row, int c, int nk, float (&f)[8]) {
-  if constexpr (VEC) {
-    if constexpr (sizeof(T) == 2) {
-      if (c < nk) unpack16<T>(ld16(row + c), *reinterpret_cast<float (*)[Vec16<T>::N]>(&f));
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; i += 4)
-        if (c + i < nk) unpack16<T>(ld16(row + c + i), *reinterpret_cast<float (*)[Vec16<T>::N]>(&f[i]));
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (c + i < nk) f[i] = to_f32<T>(row[c + i]);
-  }
-}
-
-__device__ __forceinline__ float probability(float x, float top, float inv) { return __expf(x - top) * inv; }
 
 __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
   asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
@@ -245,8 +380,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
   const uint32_t base = (raw + 1023u) & ~1023u;
   uint8_t* gen = smem_raw + (base - raw);
   volatile int* abort_flag = &abort_word;
-  const int widest = a.padded < kChunk ? a.padded : kChunk;
-  const uint32_t b_bytes = static_cast<uint32_t>(widest) * 128u;
+  const uint32_t b_bytes = static_cast<uint32_t>(a.width) * 128u;
   const uint32_t stage_bytes = 2u * kPieceBytes + 2u * b_bytes;
   const uint32_t bar0 = ptx::smem_u32(bars);
   auto ready_bar = [&](int s) { return bar0 + s * 8; };                   // the probabilities' pieces
@@ -265,7 +399,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(tfull_bar(i), 1);
-      ptx::mbar_init(tempty_bar(i), 4);
+      ptx::mbar_init(tempty_bar(i), kReaders);
     }
     abort_word = 0;
     ptx::mbar_fence_init();
@@ -290,8 +424,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
     const int j = BACKWARD ? i >> 1 : i;
     it.chunk = j % a.chunks;
     it.t0 = static_cast<int64_t>(j / a.chunks) * kTileTokens;
-    it.n0 = it.chunk * kChunk;
-    it.columns = a.padded - it.n0 < kChunk ? a.padded - it.n0 : kChunk;
+    it.n0 = it.chunk * a.width;
+    it.columns = a.padded - it.n0 < a.width ? a.padded - it.n0 : a.width;
     return it;
   };
 
@@ -355,62 +489,69 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
         __syncwarp();
       }
     }
-  } else if (warp < 6) {
+  } else if (warp < 2 + kReaders) {
     bool ok = true;
     uint32_t round = 0;
-    const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
+    const int quarter = warp & 3;         // the lanes of tensor memory that this warp may read
+    const int side = (warp - 2) / 4;      // the half of the columns
     const float unscale = a.head->unscale;
     const float scale = BACKWARD ? static_cast<float>(a.head->coef * static_cast<double>(*a.upstream)) : 0.f;
     for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x, ++round) {
       const Item it = item_of(i);
       const uint32_t acc = round & 1u;
       const int64_t t = it.t0 + quarter * 32 + lane;
+      const int c0 = side * (it.columns / 2), c1 = c0 + it.columns / 2;  // multiples of 32
       float top = 0.f, inv = 0.f, s = 0.f;
+      const T* row = static_cast<const T*>(a.logits) + t * a.ts + it.h * a.hs;
       if (t < a.ntok) {
         const float4 st = a.stats[t];
         top = it.h == 0 ? st.x : st.z;
         inv = it.h == 0 ? st.y : st.w;
-        if (BACKWARD)
-          for (int c = 0; c < a.chunks; ++c) s += a.token_s[static_cast<int64_t>(c) * a.ntok + t];
       }
       const bool live = inv != 0.f;
-      const T* row = static_cast<const T*>(a.logits) + t * a.ts + it.h * a.hs;
+      const float weight = BACKWARD ? (live ? inv * scale : 0.f) : inv * unscale;
+      Logits<T, VEC> x[4];
+      auto fetch = [&](int c) {
+#pragma unroll
+        for (int v = 0; v < 4; ++v)
+          x[v].load(row, it.n0 + c + v * 8, a.nk, live);
+      };
+      fetch(c0);
+      if (BACKWARD && t < a.ntok)
+        for (int c = 0; c < a.partials; ++c) s += a.token_s[static_cast<int64_t>(c) * a.ntok + t];
       T* out = BACKWARD ? static_cast<T*>(a.dlogits) + (t * 2 + it.h) * a.nk : nullptr;
       ok = wait(tfull_bar(acc), (round >> 1) & 1u);
       if (!ok) break;
       ptx::tc_fence_after();
       const uint32_t taddr = tmem + acc * kChunk + (static_cast<uint32_t>(quarter * 32) << 16);
-      for (int c = 0; c < it.columns; c += 32) {
-        float x[4][8];
+      for (int c = c0; c < c1; c += 32) {
+        float p[4][8];
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-#pragma unroll
-          for (int k = 0; k < 8; ++k) x[v][k] = 0.f;
-          if (live) load_logits<T, VEC>(row, it.n0 + c + v * 8, a.nk, x[v]);
-        }
+        for (int v = 0; v < 4; ++v) x[v].get(p[v]);
+        if (c + 32 < c1) fetch(c + 32);
         uint32_t r[32];
         ptx::tmem_ld_32x32(taddr + c, r);
         ptx::tmem_ld_wait(r);
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
           const int col = it.n0 + c + v * 8;
-          float o[8];
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
-            const float p = live && col + k < a.nk ? probability(x[v][k], top, inv) : 0.f;
             const float g = __uint_as_float(r[v * 8 + k]);
-            if (BACKWARD) o[k] = live ? p * fmaf(g, unscale, -s) * scale : 0.f;
-            else if (live && col + k < a.nk) s = fmaf(p, g, s);
+            const float e = exp_below(p[v][k] - top);
+            if (BACKWARD) p[v][k] = e * fmaf(g, unscale, -s) * weight;
+            else s = fmaf(e, g, s);
           }
           if (BACKWARD && t < a.ntok) {
-            if (VEC) {
+            if constexpr (VEC) {
+              constexpr int V = Vec16<T>::N;
 #pragma unroll
-              for (int k = 0; k < 8; k += Vec16<T>::N)
-                if (col + k < a.nk) *reinterpret_cast<uint4*>(out + col + k) = pack16<T>(*reinterpret_cast<float (*)[Vec16<T>::N]>(&o[k]));
+              for (int k = 0; k < 8; k += V)
+                if (col + k < a.nk) *reinterpret_cast<uint4*>(out + col + k) = pack16<T>(*reinterpret_cast<float (*)[V]>(&p[v][k]));
             } else {
 #pragma unroll
               for (int k = 0; k < 8; ++k)
-                if (col + k < a.nk) out[col + k] = from_f32<T>(o[k]);
+                if (col + k < a.nk) out[col + k] = from_f32<T>(p[v][k]);
             }
           }
         }
@@ -419,65 +560,84 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(tempty_bar(acc));
       if (!BACKWARD) {
-        s *= unscale;
-        if (t < a.ntok) a.token_s[static_cast<int64_t>(it.chunk) * a.ntok + t] = s;
+        s *= weight;
+        if (t < a.ntok) a.token_s[static_cast<int64_t>(2 * it.chunk + side) * a.ntok + t] = s;
         double all = s;
         for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(kFull, all, d);
-        if (lane == 0) a.part[static_cast<int64_t>(i) * 4 + quarter] = all;
+        if (lane == 0) a.part[static_cast<int64_t>(i) * kReaders + warp - 2] = all;
       }
     }
   } else {
     bool ok = true;
     uint32_t use = 0;
     // thread -> rows r0, r0 + 32, ... and a fixed 16-byte place (8 columns) of each 64-column block
-    const int id = threadIdx.x - 6 * 32, piece = id & 7, r0 = id >> 3;
+    const int id = threadIdx.x - (2 + kReaders) * 32, piece = id & 7, r0 = id >> 3;
     const int place = piece ^ (r0 & 7);
     constexpr int kRows = kTileTokens / (kMakers * 4);
-    for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x) {
-      const Item it = item_of(i);
-      const T* rows[kRows];
+    struct Rows {
       float top[kRows], inv[kRows];
+    };
+    Rows now, next;
+    Logits<T, VEC> x[kRows];
+    auto tokens = [&](int i, Rows& w) {
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const Item it = item_of(i);
+        const int64_t t = it.t0 + r0 + r * (kMakers * 4);
+        w.top[r] = w.inv[r] = 0.f;
+        if (i < a.items && t < a.ntok) {
+          const float4 st = a.stats[t];
+          w.top[r] = it.h == 0 ? st.z : st.x;
+          w.inv[r] = it.h == 0 ? st.w : st.y;
+        }
+      }
+    };
+    auto fetch = [&](int i, int kb, const Rows& w) {
+      const Item it = item_of(i);
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         const int64_t t = it.t0 + r0 + r * (kMakers * 4);
-        top[r] = inv[r] = 0.f;
-        rows[r] = static_cast<const T*>(a.logits) + t * a.ts + (1 - it.h) * a.hs;
-        if (t < a.ntok) {
-          const float4 st = a.stats[t];
-          top[r] = it.h == 0 ? st.z : st.x;
-          inv[r] = it.h == 0 ? st.w : st.y;
-        }
+        x[r].load(static_cast<const T*>(a.logits) + t * a.ts + (1 - it.h) * a.hs, kb * 64 + piece * 8, a.nk, w.inv[r] != 0.f);
       }
+    };
+    tokens(blockIdx.x, now);
+    fetch(blockIdx.x, 0, now);
+    for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x) {
+      tokens(i + gridDim.x, next);
       for (int kb = 0; kb < blocks; ++kb, ++use) {
         const int s = use % a.stages;
-        const int col = kb * 64 + piece * 8;
-        float x[kRows][8];
+        float p[kRows][8];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
+          x[r].get(p[r]);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) x[r][k] = 0.f;
-          if (inv[r] != 0.f) load_logits<T, VEC>(rows[r], col, a.nk, x[r]);
+          for (int k = 0; k < 8; ++k) p[r][k] = exp_below(p[r][k] - now.top[r]) * (now.inv[r] * 32768.f);
         }
+        if (kb + 1 < blocks) fetch(i, kb + 1, now);
+        else fetch(i + gridDim.x, 0, next);
         ok = wait(empty_bar(s), ((use / a.stages) & 1u) ^ 1u);
         if (!ok) break;
         uint4* dst = reinterpret_cast<uint4*>(gen + s * stage_bytes);
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-          float hi[8], lo[8];
+          uint32_t hi[4], lo[4];
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float p = inv[r] != 0.f && col + k < a.nk ? probability(x[r][k], top[r], inv[r]) * 32768.f : 0.f;
-            hi[k] = round_to<__half>(p);
-            lo[k] = p - hi[k];
+          for (int k = 0; k < 4; ++k) {
+            const __half2 h = __floats2half2_rn(p[r][2 * k], p[r][2 * k + 1]);
+            const float2 f = __half22float2(h);
+            const __half2 l = __floats2half2_rn(p[r][2 * k] - f.x, p[r][2 * k + 1] - f.y);
+            hi[k] = *reinterpret_cast<const uint32_t*>(&h);
+            lo[k] = *reinterpret_cast<const uint32_t*>(&l);
           }
           const int at = (r0 + r * (kMakers * 4)) * 8 + place;
-          dst[at] = pack16<__half>(hi);
-          dst[at + kPieceBytes / 16] = pack16<__half>(lo);
+          dst[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          dst[at + kPieceBytes / 16] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         ptx::fence_async_smem();
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(ready_bar(s));
       }
+      now = next;
     }
   }
 
@@ -497,7 +657,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
   if (!last) return;
   __threadfence();
   double v = 0.0;
-  for (int i = threadIdx.x; i < 4 * a.items; i += kProductThreads) v += static_cast<const volatile double*>(a.part)[i];
+  for (int i = threadIdx.x; i < kReaders * a.items; i += kProductThreads) v += static_cast<const volatile double*>(a.part)[i];
   for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
   if (lane == 0) sums[warp] = v;
   __syncthreads();
@@ -510,16 +670,36 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
 size_t matrix_bytes(int nk) { return static_cast<size_t>(padded_keys(nk)) * padded_keys(nk) * 2; }
 int64_t token_tiles(int64_t T) { return (T + kTileTokens - 1) / kTileTokens; }
 
-template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStream_t stream) {
+// rows made of aligned 16-byte pieces
+template <typename T> bool vector_rows(const ProductArgs& a) {
   constexpr int V = Vec16<T>::N;
-  const bool vec = a.nk % V == 0 && a.ts % V == 0 && a.hs % V == 0 && aligned16(a.logits) && (!BACKWARD || aligned16(a.dlogits));
-  const int widest = a.padded < kChunk ? a.padded : kChunk;
-  const int stage = 2 * kPieceBytes + 2 * widest * 128;
+  return a.nk % V == 0 && a.ts % V == 0 && a.hs % V == 0 && aligned16(a.logits);
+}
+
+// Columns of an item: as few as 64 while the items still fit the SMs side by side, since an item's latency is what small calls
+// cost; each item makes the probabilities of its tokens again.
+int item_width(int64_t T, int nk, int halves) {
+  const int padded = padded_keys(nk);
+  int width = padded < kChunk ? padded : kChunk;
+  for (int w = 64; w < width; w *= 2)
+    if (token_tiles(T) * ((padded + w - 1) / w) * halves <= device_sm_count()) width = w;
+  return width;
+}
+int chunks_of(int nk, int width) { return (padded_keys(nk) + width - 1) / width; }
+// what the forward leaves of s_t: a sum for each half of an item's columns
+int partial_sums(int64_t T, int nk) { return 2 * chunks_of(nk, item_width(T, nk, 1)); }
+
+template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStream_t stream) {
+  const bool vec = vector_rows<T>(a) && (!BACKWARD || aligned16(a.dlogits));
+  a.width = item_width(a.ntok, a.nk, BACKWARD ? 2 : 1);
+  a.chunks = chunks_of(a.nk, a.width);
+  a.partials = partial_sums(a.ntok, a.nk);
+  const int stage = 2 * kPieceBytes + 2 * a.width * 128;
   a.stages = 200 * 1024 / stage;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
   const int smem = a.stages * stage + 1024;
   const int64_t items = token_tiles(a.ntok) * a.chunks * (BACKWARD ? 2 : 1);
-  if (items > 0x7FFFFFFF / 4) return FMOE_ERR_UNSUPPORTED;
+  if (items > 0x7FFFFFFF / kReaders - 65536) return FMOE_ERR_UNSUPPORTED;
   a.items = static_cast<int>(items);
   const int grid = a.items < device_sm_count() ? a.items : device_sm_count();
   auto run = [&](auto* kern) -> int {
@@ -532,10 +712,10 @@ template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStrea
 
 template <typename T>
 int forward_typed(ProductArgs a, const uint8_t* mask, const int64_t* counts, Prepared* head, float4* stats, Part* part, cudaStream_t stream) {
-  const int64_t want = (a.ntok + 7) / 8, cap = static_cast<int64_t>(device_sm_count()) * 8;
+  const int64_t want = (a.ntok + 15) / 16, cap = static_cast<int64_t>(device_sm_count()) * 8;
   const int64_t grid = want > cap ? cap : want < kParts ? kParts : want;
-  balance_stats_kernel<T><<<static_cast<unsigned>(grid), 256, 0, stream>>>(static_cast<const T*>(a.logits), a.ts, a.hs, mask, a.ntok, a.nk,
-                                                                          stats, counts, part);
+  auto* kern = vector_rows<T>(a) ? balance_stats_kernel<T, true> : balance_stats_kernel<T, false>;
+  kern<<<static_cast<unsigned>(grid), 256, 0, stream>>>(static_cast<const T*>(a.logits), a.ts, a.hs, mask, a.ntok, a.nk, stats, counts, part);
   FMOE_LAUNCH_CHECK();
   const int64_t pieces = static_cast<int64_t>(a.padded) * a.padded / 4;
   FMOE_CUDA_TRY(launch_pdl(32, balance_prepare_kernel, dim3(static_cast<unsigned>((pieces + 255) / 256)), dim3(256), 0, stream, 1, counts,
@@ -549,21 +729,40 @@ int launch_expert_counts(const int64_t* indices, const uint8_t* mask, int64_t T,
                          cudaStream_t stream) {
   if (T < 0 || k < 0 || N < 0) return FMOE_ERR_BAD_ARG;
   if (N > 0 && counts == nullptr) return FMOE_ERR_BAD_ARG;
-  if (N > 0) FMOE_CUDA_TRY(cudaMemsetAsync(counts, 0, static_cast<size_t>(N) * 8, stream));
-  if (T == 0 || k == 0) return FMOE_OK;
+  if (T == 0 || k == 0) {
+    if (N > 0) FMOE_CUDA_TRY(cudaMemsetAsync(counts, 0, static_cast<size_t>(N) * 8, stream));
+    return FMOE_OK;
+  }
   if (indices == nullptr) return FMOE_ERR_BAD_ARG;
-  const int64_t want = (T * k + 255) / 256, cap = static_cast<int64_t>(device_sm_count()) * 8;
-  expert_counts_kernel<<<static_cast<unsigned>(want < cap ? want : cap), 256, 0, stream>>>(
-      indices, mask, T * k, k, N, reinterpret_cast<unsigned long long*>(counts), status);
+  unsigned long long* out = reinterpret_cast<unsigned long long*>(counts);
+  const int64_t pairs = T * k;
+  if (pairs <= 32768 && N <= 131072) {
+    const int ctas = pairs <= 4096 && N <= 16384 ? 4 : 8;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kCountThreads);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    FMOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, expert_counts_kernel<true>, indices, mask, pairs, k, N, out, status));
+    return FMOE_OK;
+  }
+  FMOE_CUDA_TRY(cudaMemsetAsync(counts, 0, static_cast<size_t>(N) * 8, stream));
+  const int64_t want = (pairs + 4 * kCountThreads - 1) / (4 * kCountThreads), cap = device_sm_count();
+  expert_counts_kernel<false><<<static_cast<unsigned>(want < cap ? want : cap), kCountThreads, 0, stream>>>(indices, mask, pairs, k, N, out, status);
   FMOE_LAUNCH_CHECK();
   return FMOE_OK;
 }
 
 size_t balance_prepared_bytes(int nk) { return nk <= 0 || nk > kMaxKeys ? 0 : kHeadBytes + 4 * matrix_bytes(nk); }
-size_t balance_stats_floats(int64_t T, int nk) { return T <= 0 || nk <= 0 || nk > kMaxKeys ? 0 : static_cast<size_t>(T) * (4 + column_chunks(nk)); }
+size_t balance_stats_floats(int64_t T, int nk) { return T <= 0 || nk <= 0 || nk > kMaxKeys ? 0 : static_cast<size_t>(T) * (4 + partial_sums(T, nk)); }
 size_t balance_workspace_bytes(int64_t T, int nk) {
   if (T < 0 || nk <= 0 || nk > kMaxKeys) return 0;
-  return kParts * sizeof(Part) + static_cast<size_t>(token_tiles(T)) * column_chunks(nk) * 4 * sizeof(double);
+  return kParts * sizeof(Part) + static_cast<size_t>(token_tiles(T)) * (partial_sums(T, nk) / 2) * kReaders * sizeof(double);
 }
 
 int launch_balance_forward(const void* logits, int64_t ts, int64_t hs, int dtype, const int64_t* counts, const uint8_t* mask, int64_t T,
@@ -595,7 +794,6 @@ int launch_balance_forward(const void* logits, int64_t ts, int64_t hs, int dtype
   a.status = status;
   a.nk = nk;
   a.padded = padded_keys(nk);
-  a.chunks = column_chunks(nk);
   float4* st = reinterpret_cast<float4*>(stats);
   switch (dtype) {
     case FMOE_DTYPE_F32: return forward_typed<float>(a, mask, counts, head, st, part, stream);
@@ -628,7 +826,6 @@ int launch_balance_backward(const void* logits, int64_t ts, int64_t hs, int dtyp
   a.status = status;
   a.nk = nk;
   a.padded = padded_keys(nk);
-  a.chunks = column_chunks(nk);
   switch (dtype) {
     case FMOE_DTYPE_F32: return launch_product<float, true>(a, stream);
     case FMOE_DTYPE_BF16: return launch_product<__nv_bfloat16, true>(a, stream);

@@ -3,12 +3,13 @@ in 8 bits for a product that takes one (the reference leaves both to its caller)
 
 from __future__ import annotations
 
+import functools
 from typing import Optional, Tuple
 
 import torch
 
 from .. import _lib
-from .utils import contiguous, plain_call
+from .utils import backward_once, contiguous, plain_call
 
 MAX_HIDDEN = 16384
 
@@ -16,16 +17,17 @@ MAX_HIDDEN = 16384
 def _arguments(x, residual, weight, eps):
     """Device, contiguous tensors, rows and columns of a call."""
     dev = _lib.require_cuda(x, residual, weight)
-    if x.dim() == 0 or not 0 < x.shape[-1] <= MAX_HIDDEN:
+    shape = x.shape
+    if not shape or not 0 < shape[-1] <= MAX_HIDDEN:
         raise _lib.FmoeError(f"expected x[..., hidden] with 1 to {MAX_HIDDEN} columns")
-    H = x.shape[-1]
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
+    H = shape[-1]
+    if residual is not None and (residual.shape != shape or residual.dtype != x.dtype):
         raise _lib.FmoeError("residual must match x in shape and dtype")
     if weight is not None and (weight.shape != (H,) or weight.dtype != x.dtype):
         raise _lib.FmoeError("weight must be a [hidden] tensor in the dtype of x")
     if not eps >= 0:
         raise _lib.FmoeError("eps must not be negative")
-    return dev, contiguous(x), contiguous(residual), contiguous(weight), x.numel() // H, H
+    return dev, x.contiguous(), contiguous(residual), contiguous(weight), x.numel() // H, H
 
 
 def _forward(x, residual, weight, eps):
@@ -39,21 +41,24 @@ def _forward(x, residual, weight, eps):
     return normed, summed
 
 
+_workspace_bytes = functools.lru_cache(maxsize=256)(lambda *shape: _lib.lib().fmoe_add_rms_norm_backward_workspace_bytes(*shape))
+
+
 def _backward(dnormed, dsummed, summed, weight, eps, want_dweight):
     """(dx, dweight): the gradient of the sum, which x and the residual share, and of the weight."""
-    dev = _lib.require_cuda(dnormed, dsummed, summed, weight)
-    # addresses go to the library: hooks may return saved tensors with other strides
-    dn, ds, s, w = (contiguous(t if t is None or t.dtype == summed.dtype else t.to(summed.dtype))
-                    for t in (dnormed, dsummed, summed, weight))
-    H = s.shape[-1]
+    # addresses go to the library: gradients may be views, and hooks may return saved tensors with other strides
+    s, w = summed.contiguous(), contiguous(weight)
+    dn, ds = (t if t is None or t.dtype == s.dtype else t.to(s.dtype) for t in (dnormed, dsummed))
+    dn, ds = dn.contiguous(), contiguous(ds)
+    dev, H = s.device, s.shape[-1]
     rows, code = s.numel() // H, _lib.dtype_code(s)
     dx = torch.empty_like(s)
     dw = ws = None
     nbytes = 0
     if want_dweight:
-        dw = s.new_empty(H)
-        nbytes = _lib.lib().fmoe_add_rms_norm_backward_workspace_bytes(rows, H, code)
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=dev)
+        dw = torch.empty_like(w)
+        nbytes = _workspace_bytes(rows, H, code)
+        ws = s.new_empty(nbytes, dtype=torch.uint8)
     rc = _lib.call("fmoe_add_rms_norm_backward", dev, dn.data_ptr(), _lib.ptr(ds), s.data_ptr(), _lib.ptr(w), dx.data_ptr(),
                    _lib.ptr(dw), code, rows, H, eps, _lib.ptr(ws), nbytes)
     if rc:
@@ -66,14 +71,13 @@ class AddRMSNormFunc(torch.autograd.Function):
     def forward(ctx, x, residual, weight, eps):
         normed, summed = _forward(x, residual, weight, eps)
         ctx.eps = eps
-        ctx.with_residual = residual is not None
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(summed, weight)
         # without a residual the sum is x itself, which the caller has
         return (normed, summed) if residual is not None else normed
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @backward_once
     def backward(ctx, dnormed, dsummed=None):
         summed, weight = ctx.saved_tensors
         dw = None
@@ -81,7 +85,7 @@ class AddRMSNormFunc(torch.autograd.Function):
             dx = dsummed
         else:
             dx, dw = _backward(dnormed, dsummed, summed, weight, ctx.eps, ctx.needs_input_grad[2])
-        return dx, dx if ctx.with_residual else None, dw, None
+        return dx, dx if ctx.needs_input_grad[1] else None, dw, None
 
 
 def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
@@ -107,14 +111,15 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor] = None, w
     ``quantised`` is float8_e4m3fn in the shape of x; ``scales`` is float32, ``[..., 1]`` for one scale a row (``group_size=None``)
     or ``[..., ceil(hidden / group_size)]`` for one scale for each 32, 64 or 128 columns: the largest absolute value of the row or
     block / 448 (at least 2^-126).  The float32 value is rounded once, to 8 bits."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight)):
+    if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad
+                                    or weight is not None and weight.requires_grad):
         raise _lib.FmoeError("add_rms_norm_fp8 has no gradient: call it under torch.no_grad(), or add_rms_norm")
     if group_size not in (None, 32, 64, 128):
         raise _lib.FmoeError("group_size must be None, 32, 64 or 128")
     eps = float(eps)
     dev, x, r, w, rows, H = _arguments(x, residual, weight, eps)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    scales = torch.empty((*x.shape[:-1], 1 if group_size is None else -(-H // group_size)), dtype=torch.float32, device=dev)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scales = x.new_empty((*x.shape[:-1], 1 if group_size is None else -(-H // group_size)), dtype=torch.float32)
     summed = x if r is None else torch.empty_like(x)
     rc = _lib.call("fmoe_add_rms_norm_fp8", dev, x.data_ptr(), _lib.ptr(r), _lib.ptr(w), None if r is None else summed.data_ptr(),
                    q.data_ptr(), scales.data_ptr(), _lib.dtype_code(x), rows, H, group_size or 0, eps)

@@ -3,12 +3,13 @@ in ``last_indices`` (the reference leaves both to its caller)."""
 
 from __future__ import annotations
 
+import functools
 from typing import Optional
 
 import torch
 
 from .. import _lib
-from .utils import contiguous, plain_call
+from .utils import backward_once, contiguous, plain_call
 
 MAX_KEYS = 2048
 
@@ -38,7 +39,7 @@ def expert_counts(indices: torch.Tensor, num_experts: int, token_mask: Optional[
     idx = contiguous(indices)
     if idx.dtype != torch.int64:
         idx = idx.to(torch.int64)
-    counts = torch.empty(num_experts, dtype=torch.int64, device=dev)
+    counts = idx.new_empty(num_experts)
     rc = _lib.call("fmoe_expert_counts", dev, idx.data_ptr(), _lib.ptr(mask), T, k, num_experts, counts.data_ptr(),
                    _lib.status_ptr(dev))
     if rc:
@@ -53,32 +54,41 @@ def _strided(logits):
     return logits, logits.stride(1), logits.stride(0)
 
 
+@functools.lru_cache(maxsize=256)
+def _layout(T, nk):
+    """Bytes of (what the backward needs of the counts, of the tokens, scratch), each rounded up to 256."""
+    L = _lib.lib()
+    sizes = L.fmoe_balance_loss_prepared_bytes(nk), 4 * L.fmoe_balance_loss_stats_floats(T, nk), L.fmoe_balance_loss_workspace_bytes(T, nk)
+    return [(n + 255) // 256 * 256 for n in sizes]
+
+
 def _loss_forward(logits, counts, mask):
+    """(loss, state): the state is one allocation, for the backward."""
     dev = logits.device
     _, T, nk = logits.shape
-    L = _lib.lib()
     logits, ts, hs = _strided(logits)
-    loss = torch.empty((), dtype=torch.float32, device=dev)
-    stats = torch.empty(L.fmoe_balance_loss_stats_floats(T, nk), dtype=torch.float32, device=dev)
-    prepared = torch.empty(L.fmoe_balance_loss_prepared_bytes(nk), dtype=torch.uint8, device=dev)
-    ws = torch.empty(L.fmoe_balance_loss_workspace_bytes(T, nk), dtype=torch.uint8, device=dev)
+    prepared, stats, scratch = _layout(T, nk)
+    loss = counts.new_empty((), dtype=torch.float32)
+    state = counts.new_empty(prepared + stats + scratch, dtype=torch.uint8)
+    at = state.data_ptr()
     rc = _lib.call("fmoe_balance_loss_forward", dev, logits.data_ptr(), ts, hs, _lib.dtype_code(logits), counts.data_ptr(),
-                   _lib.ptr(mask), T, nk, loss.data_ptr(), stats.data_ptr(), prepared.data_ptr(), prepared.numel(), ws.data_ptr(),
-                   ws.numel(), _lib.status_ptr(dev))
+                   _lib.ptr(mask), T, nk, loss.data_ptr(), at + prepared, at, prepared, at + prepared + stats, scratch,
+                   _lib.status_ptr(dev))
     if rc:
         _lib.check(rc, "fmoe_balance_loss_forward")
-    return loss, stats, prepared
+    return loss, state
 
 
-def _loss_backward(logits, stats, prepared, upstream):
+def _loss_backward(logits, state, upstream):
     dev = logits.device
     _, T, nk = logits.shape
     logits, ts, hs = _strided(logits)
+    prepared = _layout(T, nk)[0]
     # the rows of both halves of a token next to each other, as the router's product writes its logits
-    dlogits = torch.empty((T, 2, nk), dtype=logits.dtype, device=dev)
-    rc = _lib.call("fmoe_balance_loss_backward", dev, logits.data_ptr(), ts, hs, _lib.dtype_code(logits), T, nk,
-                   stats.data_ptr(), prepared.data_ptr(), prepared.numel(), upstream.data_ptr(), dlogits.data_ptr(),
-                   _lib.status_ptr(dev))
+    dlogits = logits.new_empty((T, 2, nk))
+    at = state.data_ptr()
+    rc = _lib.call("fmoe_balance_loss_backward", dev, logits.data_ptr(), ts, hs, _lib.dtype_code(logits), T, nk, at + prepared, at,
+                   prepared, upstream.data_ptr(), dlogits.data_ptr(), _lib.status_ptr(dev))
     if rc:
         _lib.check(rc, "fmoe_balance_loss_backward")
     return dlogits.transpose(0, 1)
@@ -87,18 +97,15 @@ def _loss_backward(logits, stats, prepared, upstream):
 class BalanceLossFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, router_logits, counts, mask):
-        loss, stats, prepared = _loss_forward(router_logits, counts, mask)
-        ctx.save_for_backward(router_logits, stats, prepared)
+        loss, state = _loss_forward(router_logits, counts, mask)
+        ctx.save_for_backward(router_logits, state)
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @backward_once
     def backward(ctx, upstream):
-        logits, stats, prepared = ctx.saved_tensors
-        if not ctx.needs_input_grad[0]:
-            return None, None, None
-        upstream = upstream.to(torch.float32).contiguous()
-        return _loss_backward(logits, contiguous(stats), contiguous(prepared), upstream), None, None
+        logits, state = ctx.saved_tensors
+        return _loss_backward(logits, state.contiguous(), upstream if upstream.dtype == torch.float32 else upstream.to(torch.float32)), None, None
 
 
 def balance_loss(router_logits: torch.Tensor, counts: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:

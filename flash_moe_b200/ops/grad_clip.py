@@ -3,6 +3,7 @@ is one of the longer ones of a training step (the reference leaves it to its cal
 
 from __future__ import annotations
 
+import functools
 from array import array
 from typing import Iterable, List, Union
 
@@ -24,7 +25,7 @@ def _dense(t: torch.Tensor) -> bool:
 
 
 def _call(name, grads: List[torch.Tensor], head, grad_scale) -> torch.Tensor:
-    dev = _lib.require_cuda(*grads)
+    dev = grads[0].device
     scale, device_scale = grad_scale, None
     if isinstance(grad_scale, torch.Tensor):
         if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
@@ -33,12 +34,17 @@ def _call(name, grads: List[torch.Tensor], head, grad_scale) -> torch.Tensor:
     elif not 0 <= grad_scale < float("inf"):
         raise _lib.FmoeError("grad_scale must be a finite number that is not negative")
     n = len(grads)
+    try:
+        codes = array("i", [_lib.DTYPE_CODE[g.dtype] for g in grads])
+    except KeyError:
+        for g in grads:
+            _lib.dtype_code(g)  # raises for the one that is not supported
+        raise
     ptrs = array("Q", [g.data_ptr() for g in grads])
     numels = array("q", [g.numel() for g in grads])
-    codes = array("i", [_lib.dtype_code(g) for g in grads])
-    norm = torch.empty((), dtype=torch.float32, device=dev)
-    nbytes = _lib.lib().fmoe_grad_norm_workspace_bytes(n)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    norm = grads[0].new_empty((), dtype=torch.float32)
+    nbytes = _workspace_bytes(n)
+    ws = grads[0].new_empty(nbytes, dtype=torch.uint8)
     rc = _lib.call(name, dev, ptrs.buffer_info()[0], numels.buffer_info()[0], codes.buffer_info()[0], n, *head, scale, device_scale,
                    norm.data_ptr(), ws.data_ptr(), nbytes)
     if rc == _lib.ERR_BAD_ARG:
@@ -48,14 +54,29 @@ def _call(name, grads: List[torch.Tensor], head, grad_scale) -> torch.Tensor:
     return norm
 
 
-def _once(tensors: Iterable[torch.Tensor]) -> List[torch.Tensor]:
-    """Each tensor that has values once, however often it is given."""
-    seen = {}
+_workspace_bytes = functools.lru_cache(maxsize=256)(lambda n: _lib.lib().fmoe_grad_norm_workspace_bytes(n))
+
+
+def _once(tensors: Iterable[torch.Tensor], what: str) -> List[torch.Tensor]:
+    """Each tensor that has values once, however often it is given; all on one CUDA device and dense (`what`: the refusal of
+    others, or "" where a copy will do)."""
+    seen, dev = {}, None
     for t in tensors:
-        if t.is_sparse or t.layout != torch.strided:
+        if t.layout is not torch.strided:
             raise _lib.FmoeError("sparse gradients are not supported")
-        if t.numel():
-            seen.setdefault((t.data_ptr(), t.numel(), t.dtype), t)
+        n = t.numel()
+        if not n:
+            continue
+        if dev is None:
+            dev = _lib.require_cuda(t)
+        elif t.device != dev:
+            _lib.require_cuda(t)
+            raise _lib.FmoeError(f"tensors on different devices: {dev} and {t.device}")
+        if not t.is_contiguous() and not _dense(t):
+            if what:
+                raise _lib.FmoeError(what)
+            t = t.contiguous()
+        seen.setdefault((t.data_ptr(), n, t.dtype), t)
     return list(seen.values())
 
 
@@ -63,10 +84,10 @@ def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], grad_scale: 
     """``grad_scale * sqrt(sum of all squares)`` over all tensors, a float32 scalar on their device (no synchronisation).  A tensor
     given twice counts once."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
-    grads = _once(t.detach() for t in tensors)
+    grads = _once((t.detach() for t in tensors), "")
     if not grads:
         return torch.zeros((), device=tensors[0].device if tensors else None)
-    return _call("fmoe_grad_norm", [g if _dense(g) else g.contiguous() for g in grads], (), grad_scale)
+    return _call("fmoe_grad_norm", grads, (), grad_scale)
 
 
 def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max_norm: float,
@@ -82,11 +103,10 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     if not max_norm >= 0 or not eps >= 0:
         raise _lib.FmoeError("max_norm and eps must not be negative")
-    grads = _once(p.grad for p in parameters if p.grad is not None)
+    grads = _once([g for g in [p.grad for p in parameters] if g is not None],
+                  "a gradient with gaps or repeated values cannot be scaled in place: make it contiguous")
     if not grads:
         return torch.zeros((), device=parameters[0].device if parameters else None)
-    if not all(_dense(g) for g in grads):
-        raise _lib.FmoeError("a gradient with gaps or repeated values cannot be scaled in place: make it contiguous")
     norm = _call("fmoe_clip_grad_norm", grads, (max_norm, eps), grad_scale)
     torch.autograd.graph.increment_version(grads)
     return norm

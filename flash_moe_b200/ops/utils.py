@@ -19,3 +19,14 @@ def plain_call() -> bool:
     recorded, no forward-mode level is open (the node is what refuses tangents, which would be dropped silently) and
     torch.jit is not tracing (the node is what a trace records)."""
     return not _grad_enabled() and forward_ad._current_level < 0 and not _tracing()
+
+
+def backward_once(backward):
+    """``once_differentiable`` for the backward of an op: a second differentiation is refused.  Where no graph of the backward is
+    recorded, which is nearly always, its bookkeeping (4 us of host time) is left out."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if _grad_enabled() else backward(ctx, *grads)
+
+    return run

@@ -1,9 +1,13 @@
 """`expert_counts` and `balance_loss` against the formulas in 64 bits, the latter over the whole [T, num_experts] probabilities.
 
-u = 2^-24 is half a step of float32.  A probability comes from a few float32 operations (expf is within 2 ulp, a sum over nk
-values, a division): off by less than (nk / 32 + 16) u.  The products with the centred counts are sums of nk terms: off by nk u of
-the sum of their absolute values, plus what the probabilities are off.  So G_h is off by (2 nk + 32) u of p |C - mean|, which bounds
-what the differences G_h - s and the loss are off; half a step of the gradient's type comes on top."""
+u = 2^-24 is half a step of float32.  A probability e^t / sum, t = x - max, comes from a few float32 operations, a sum over nk
+values and the exponential of base 2 at t log2 e.  That product is rounded, by at most |t| log2 e u, which is |t| u of the
+exponential: nothing for the keys that matter, more than its other errors together where the probability is below e^-16.  So p is
+off by less than (nk / 32 + 16 + |t|) u of itself.  The products with the centred counts are sums of nk terms: off by nk u of the
+sum of their absolute values, plus what the probabilities are off, where the |t| weigh in with sum p |t| <= sum p ln(1 / p) <= ln nk,
+less than 8.  So G_h is off by (2 nk + 32) u of p |C - mean|, which bounds what the differences G_h - s and the loss are off; a
+gradient, p (G - s), is off by |t| u of p (|G| + |s|) more; half a step of its type comes on top.  The exponential is 0 where it
+would be below 2^-126, the smallest normal float32: that much of |G| + |s| a gradient may be off as well."""
 
 import math
 
@@ -112,8 +116,10 @@ def reference(logits, counts, mask, upstream):
     bound = torch.stack([p[1] @ d.t(), p[0] @ d])
     s = (p[0] * bound[0]).sum(-1)
     unit = (2 * nk + 32) * U * nk * nk / total
-    slack[:, keep] = abs(upstream) / tokens * unit * p * (bound + s[None, :, None])
-    return float(loss), unit * float(s.mean()) + U * float(loss), dlogits, slack
+    t = (rows.detach().amax(-1, keepdim=True) - rows.detach()).clamp(max=750.0)  # e^-750 is 0 in 64 bits too
+    own = (2 * nk + 32 + t) * U * nk * nk / total
+    slack[:, keep] = abs(upstream) / tokens * (own * p + 2.0**-126 * nk * nk / total) * (bound + s[None, :, None])
+    return loss.item(), unit * float(s.mean()) + U * loss.item(), dlogits, slack
 
 
 def check(T, nk, k, dtype, masked=0.0, seed=0, upstream=1.0, counts=None, logits=None):
