@@ -15,6 +15,8 @@
 // Launches: row statistics (maximum and 1 / sum of both halves) beside the sums of the counts; the centred counts as float16
 // pieces in the order in which shared memory wants them; the product with s_t and the loss; for the gradient one more product
 // kernel, which needs nothing from memory but the logits, five numbers a token and the pieces.
+#include <cstring>
+
 #include "common.cuh"
 #include "ptx_sm100.cuh"
 
@@ -53,6 +55,44 @@ __device__ __forceinline__ void count_one(int64_t e, int64_t N, int* ids, unsign
   atomicAdd(counts + e, 1ull);
 }
 
+// Walks over selections i, i + step, ...: reads kAhead ids, and the mask of their tokens, before the first is used.  The token moves
+// on by whole and left-over slots, without a division a selection.
+template <int kAhead, typename Use>
+__device__ __forceinline__ void each_selection(const int64_t* indices, const uint8_t* mask, int64_t i, int64_t end, int64_t step, int k,
+                                               Use&& use) {
+  int64_t token = 0, tokens = 0;
+  int slot = 0, slots = 0;
+  if (mask != nullptr) {
+    token = i / k;
+    slot = static_cast<int>(i % k);
+    tokens = step / k;
+    slots = static_cast<int>(step % k);
+  }
+  while (i < end) {
+    int64_t e[kAhead];
+    uint8_t keep[kAhead];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const bool in = i + u * step < end;
+      e[u] = in ? indices[i + u * step] : -1;
+      keep[u] = 1;
+      if (mask != nullptr) {
+        if (in) keep[u] = mask[token];
+        token += tokens;
+        slot += slots;
+        if (slot >= k) {
+          slot -= k;
+          ++token;
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+      if (keep[u] != 0) use(e[u]);
+    i += kAhead * step;
+  }
+}
+
 // One cluster of CTAs clears the counts itself where the call is small: a launch less.
 template <bool CLEAR>
 __global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const int64_t* indices, const uint8_t* mask, int64_t pairs, int k,
@@ -70,21 +110,55 @@ __global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const int6
   } else {
     __syncthreads();
   }
-  constexpr int kAhead = 4;
-  for (int64_t i0 = first; i0 < pairs; i0 += kAhead * step) {
-    int64_t e[kAhead];
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int64_t i = i0 + u * step;
-      e[u] = -1;
-      if (i < pairs && (mask == nullptr || mask[pairs <= 0xFFFFFFFFll ? static_cast<uint32_t>(i) / static_cast<uint32_t>(k) : i / k] != 0)) e[u] = indices[i];
-    }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) count_one(e[u], N, ids, seen, counts, status);
-  }
+  each_selection<4>(indices, mask, first, pairs, step, k, [&](int64_t e) { count_one(e, N, ids, seen, counts, status); });
   __syncthreads();
   for (int i = threadIdx.x; i < kCountPlaces; i += kCountThreads)
     if (seen[i] != 0) atomicAdd(counts + ids[i], static_cast<unsigned long long>(seen[i]));
+}
+
+// Many selections of not too many experts: every CTA counts all its selections in shared memory, in 16 bits an expert, and the
+// eight CTAs of a cluster add theirs up before they go to global memory, each a part of the experts and in ascending order.
+// At 4.2 million selections of 65536 experts the tables above are mostly taken by others: 47 us, by this kernel XX.
+constexpr int kHistCtas = 8;
+constexpr int kHistThreads = 1024;
+constexpr int kHistExperts = 102400;      // 200 KB
+constexpr int64_t kHistMost = 65535;      // selections of a CTA before a counter could overflow
+
+__device__ __forceinline__ unsigned ld_cluster_u16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared::cluster.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
+}
+
+__global__ void __launch_bounds__(kHistThreads, 1) expert_histogram_kernel(const int64_t* indices, const uint8_t* mask, int64_t pairs, int k,
+                                                                           int N, unsigned long long* counts, int32_t* status) {
+  extern __shared__ uint4 hist[];
+  unsigned* words = reinterpret_cast<unsigned*>(hist);
+  const int quads = (N + 7) / 8;  // 16 bytes, eight experts
+  const uint32_t rank = ptx::cluster_ctarank();
+  const int64_t p0 = pairs * blockIdx.x / gridDim.x, p1 = pairs * (blockIdx.x + 1) / gridDim.x;
+  // all CTAs of a cluster go round equally often
+  const int64_t most = pairs / gridDim.x + 1;
+  for (int64_t done = 0; done < most; done += kHistMost) {
+    for (int i = threadIdx.x; i < quads; i += kHistThreads) hist[i] = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+    const int64_t end = p0 + done + kHistMost < p1 ? p0 + done + kHistMost : p1;
+    each_selection<8>(indices, mask, p0 + done + threadIdx.x, end, kHistThreads, k, [&](int64_t e) {
+      if (e >= 0 && e < N) atomicAdd(words + (e >> 1), 1u << ((e & 1) * 16));
+      else if (e != -1 && status != nullptr) atomicOr(status, FMOE_STATUS_BAD_EXPERT_ID);
+    });
+    ptx::cluster_sync();
+    // a lane per expert: a warp adds to 256 consecutive bytes, a quarter of the sectors that a lane per 16 bytes would touch
+    const int e0 = N * static_cast<int64_t>(rank) / kHistCtas, e1 = N * static_cast<int64_t>(rank + 1) / kHistCtas;
+    const uint32_t base = ptx::smem_u32(hist);
+    for (int e = e0 + threadIdx.x; e < e1; e += kHistThreads) {
+      unsigned sum = 0;
+#pragma unroll
+      for (int r = 0; r < kHistCtas; ++r) sum += ld_cluster_u16(ptx::map_to_cta(base + e * 2, r));
+      if (sum != 0) atomicAdd(counts + e, static_cast<unsigned long long>(sum));
+    }
+    ptx::cluster_sync();  // nobody clears, or leaves, while others read
+  }
 }
 
 // ------------------------------------------------------------------------------------------------ statistics and counts
@@ -122,42 +196,39 @@ template <typename T> __device__ __forceinline__ uint32_t minus_infinity() { ret
 template <> __device__ __forceinline__ uint32_t minus_infinity<__nv_bfloat16>() { return 0xFF80FF80u; }
 template <> __device__ __forceinline__ uint32_t minus_infinity<__half>() { return 0xFC00FC00u; }
 
-// Eight logits of a row from column c on, as they are loaded.  What lies behind the row's end, or in a row that is not read, is
-// minus infinity: its exponential is 0 and no use of the values has to ask.
-template <typename T, bool VEC> struct Logits;
-template <typename T> struct Logits<T, true> {  // rows made of aligned 16-byte pieces
-  static constexpr int kLoads = 8 / Vec16<T>::N;
-  uint4 q[kLoads];
-  __device__ __forceinline__ void load(const T* row, int c, int nk, bool read = true) {
-    const uint32_t none = minus_infinity<T>();
+// Pieces of a row: 16 bytes, 8 or 4 logits, from column c on.  What lies behind the row's end, or in a row that is not read, is
+// minus infinity: its exponential is 0 and no use of the values has to ask.  VEC: rows are made of aligned pieces.
+template <typename T, bool VEC> __device__ __forceinline__ uint4 load_piece(const T* row, int c, int nk, bool read = true) {
+  constexpr int N = Vec16<T>::N;
+  const uint32_t none = minus_infinity<T>();
+  uint4 q = make_uint4(none, none, none, none);
+  if constexpr (VEC) {
+    if (read && c < nk) q = ld16(row + c);
+  } else {
+    T v[N];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      q[i] = make_uint4(none, none, none, none);
-      if (read && c + i * Vec16<T>::N < nk) q[i] = ld16(row + c + i * Vec16<T>::N);
-    }
+    for (int i = 0; i < N; ++i) v[i] = read && c + i < nk ? row[c + i] : from_f32<T>(-INFINITY);
+    memcpy(&q, v, 16);
   }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+  return q;
+}
+template <typename T, bool VEC> __device__ __forceinline__ void store_piece(T* row, int c, int nk, const uint4& q) {
+  constexpr int N = Vec16<T>::N;
+  if constexpr (VEC) {
+    if (c < nk) *reinterpret_cast<uint4*>(row + c) = q;
+  } else {
+    T v[N];
+    memcpy(v, &q, 16);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) unpack16<T>(q[i], *reinterpret_cast<float (*)[Vec16<T>::N]>(&f[i * Vec16<T>::N]));
+    for (int i = 0; i < N; ++i)
+      if (c + i < nk) row[c + i] = v[i];
   }
-};
-template <typename T> struct Logits<T, false> {
-  T v[8];
-  __device__ __forceinline__ void load(const T* row, int c, int nk, bool read = true) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      v[i] = from_f32<T>(-INFINITY);
-      if (read && c + i < nk) v[i] = row[c + i];
-    }
-  }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = to_f32<T>(v[i]);
-  }
-};
+}
 
 // (maximum, 1 / sum of exp(x - maximum)) of each half; 0, 0 for masked tokens, which are not read: no sum has an inverse of 0
-template <typename T, bool VEC>
+// Eight lanes share a row, so a warp has four tokens at a time and a lane enough values for its part of the reductions.  HELD: the
+// 16-byte pieces that a lane holds of each half; what longer rows have beside them is read again for the sum.
+template <typename T, bool VEC, int HELD>
 __global__ void __launch_bounds__(256) balance_stats_kernel(const T* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok,
                                                             int nk, float4* stats, const int64_t* counts, Part* part) {
   pdl_launch_dependents();
@@ -196,69 +267,59 @@ __global__ void __launch_bounds__(256) balance_stats_kernel(const T* logits, int
       part[blockIdx.x] = {c, top, mask != nullptr ? m : blockIdx.x == 0 ? static_cast<long long>(ntok) : 0ll};
     }
   }
-  // A warp takes kRows tokens at a time.  A lane holds eight values of each row and 256 columns; longer rows are read again for
-  // the sum.
-  constexpr int kRows = 2;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * 8 * kRows;
-  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * kRows; t0 < ntok; t0 += step) {
-    Logits<T, VEC> x[kRows][2];
-    float top[2 * kRows], sum[2 * kRows];
-    bool live[kRows];
+  constexpr int N = Vec16<T>::N;
+  const int sub = lane & 7;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 32;
+  for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * 4; t0 < ntok; t0 += step) {
+    const int64_t t = t0 + (lane >> 3);
+    const bool live = t < ntok && (mask == nullptr || mask[t] != 0);
+    const T* row[2] = {logits + t * ts, logits + t * ts + hs};
+    uint4 q[2][HELD];
 #pragma unroll
-    for (int r = 0; r < kRows; ++r) live[r] = t0 + r < ntok && (mask == nullptr || mask[t0 + r] != 0);
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+      for (int u = 0; u < HELD; ++u) q[h][u] = load_piece<T, VEC>(row[h], (u * 8 + sub) * N, nk, live);
+    float top[2], sum[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) x[r][h].load(logits + (t0 + r) * ts + h * hs, lane * 8, nk, live[r]);
+    for (int h = 0; h < 2; ++h) {
+      top[h] = -INFINITY;
+      auto join = [&](const uint4& v) {
+        float f[N];
+        unpack16<T>(v, f);
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+        for (int i = 0; i < N; ++i) top[h] = fmaxf(top[h], f[i]);
+      };
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float f[8], m;
-        x[r][h].get(f);
-        m = fmaxf(fmaxf(fmaxf(f[0], f[1]), fmaxf(f[2], f[3])), fmaxf(fmaxf(f[4], f[5]), fmaxf(f[6], f[7])));
-        if (live[r])
-          for (int c = (32 + lane) * 8; c < nk; c += 256) {
-            Logits<T, VEC> y;
-            y.load(logits + (t0 + r) * ts + h * hs, c, nk);
-            y.get(f);
+      for (int u = 0; u < HELD; ++u) join(q[h][u]);
+      if (live)
+        for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) join(load_piece<T, VEC>(row[h], c, nk));
+    }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) m = fmaxf(m, f[i]);
-          }
-        top[2 * r + h] = m;
-      }
+    for (int d = 4; d > 0; d >>= 1) {
+      top[0] = fmaxf(top[0], __shfl_xor_sync(kFull, top[0], d));
+      top[1] = fmaxf(top[1], __shfl_xor_sync(kFull, top[1], d));
+    }
 #pragma unroll
-    for (int d = 16; d > 0; d >>= 1)
+    for (int h = 0; h < 2; ++h) {
+      sum[h] = 0.f;
+      auto join = [&](const uint4& v) {
+        float f[N];
+        unpack16<T>(v, f);
 #pragma unroll
-      for (int i = 0; i < 2 * kRows; ++i) top[i] = fmaxf(top[i], __shfl_xor_sync(kFull, top[i], d));
+        for (int i = 0; i < N; ++i) sum[h] += exp_below(f[i] - top[h]);
+      };
 #pragma unroll
-    for (int r = 0; r < kRows; ++r)
+      for (int u = 0; u < HELD; ++u) join(q[h][u]);
+      if (live)
+        for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) join(load_piece<T, VEC>(row[h], c, nk));
+    }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float f[8], v = 0.f;
-        const float m = top[2 * r + h];
-        x[r][h].get(f);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v += exp_below(f[i] - m);
-        if (live[r])
-          for (int c = (32 + lane) * 8; c < nk; c += 256) {
-            Logits<T, VEC> y;
-            y.load(logits + (t0 + r) * ts + h * hs, c, nk);
-            y.get(f);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v += exp_below(f[i] - m);
-          }
-        sum[2 * r + h] = v;
-      }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1)
-#pragma unroll
-      for (int i = 0; i < 2 * kRows; ++i) sum[i] += __shfl_xor_sync(kFull, sum[i], d);
-#pragma unroll
-    for (int r = 0; r < kRows; ++r)
-      if (lane == r && t0 + r < ntok)
-        stats[t0 + r] = live[r] ? make_float4(top[2 * r], 1.f / sum[2 * r], top[2 * r + 1], 1.f / sum[2 * r + 1])
-                                : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int d = 4; d > 0; d >>= 1) {
+      sum[0] += __shfl_xor_sync(kFull, sum[0], d);
+      sum[1] += __shfl_xor_sync(kFull, sum[1], d);
+    }
+    if (sub == 0 && t < ntok)
+      stats[t] = live ? make_float4(top[0], 1.f / sum[0], top[1], 1.f / sum[1]) : make_float4(0.f, 0.f, 0.f, 0.f);
   }
 }
 
@@ -343,6 +404,7 @@ constexpr int kMakers = 8, kReaders = 8;  // warps
 constexpr int kProductThreads = (2 + kReaders + kMakers) * 32;
 constexpr int kPieceBytes = kTileTokens * 128;  // one piece of the probabilities
 constexpr int kMaxStages = 4;
+constexpr int kTurnPieces = 32 * 5;  // shared memory of a reading warp, in 16-byte pieces
 
 struct ProductArgs {
   const void* logits;
@@ -492,8 +554,12 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
   } else if (warp < 2 + kReaders) {
     bool ok = true;
     uint32_t round = 0;
-    const int quarter = warp & 3;         // the lanes of tensor memory that this warp may read
-    const int side = (warp - 2) / 4;      // the half of the columns
+    const int quarter = warp & 3;     // the lanes of tensor memory that this warp may read
+    const int side = (warp - 2) / 4;  // the half of the columns
+    // 64 bytes of 32 rows at a time.  Memory is read and written with four lanes on a row, eight lines to an instruction; a
+    // thread per row would touch 32.  The chunk changes hands in shared memory, rows 80 bytes apart.
+    constexpr int N = Vec16<T>::N, kColumns = 4 * N;
+    uint4* turn = reinterpret_cast<uint4*>(gen + a.stages * stage_bytes) + (warp - 2) * kTurnPieces;
     const float unscale = a.head->unscale;
     const float scale = BACKWARD ? static_cast<float>(a.head->coef * static_cast<double>(*a.upstream)) : 0.f;
     for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x, ++round) {
@@ -502,58 +568,73 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
       const int64_t t = it.t0 + quarter * 32 + lane;
       const int c0 = side * (it.columns / 2), c1 = c0 + it.columns / 2;  // multiples of 32
       float top = 0.f, inv = 0.f, s = 0.f;
-      const T* row = static_cast<const T*>(a.logits) + t * a.ts + it.h * a.hs;
       if (t < a.ntok) {
         const float4 st = a.stats[t];
         top = it.h == 0 ? st.x : st.z;
         inv = it.h == 0 ? st.y : st.w;
       }
-      const bool live = inv != 0.f;
-      const float weight = BACKWARD ? (live ? inv * scale : 0.f) : inv * unscale;
-      Logits<T, VEC> x[4];
+      const float weight = BACKWARD ? (inv != 0.f ? inv * scale : 0.f) : inv * unscale;
+      // the lane's part of a chunk in memory: piece lane % 4 of the rows lane / 4 + 8 u
+      const int64_t first = it.t0 + quarter * 32 + (lane >> 2);
+      const T* rows = static_cast<const T*>(a.logits) + first * a.ts + it.h * a.hs;
+      T* outs = BACKWARD ? static_cast<T*>(a.dlogits) + (first * 2 + it.h) * a.nk : nullptr;
+      bool live[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) live[u] = __shfl_sync(kFull, inv, (lane >> 2) + 8 * u) != 0.f;
+      uint4 q[4];
       auto fetch = [&](int c) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v)
-          x[v].load(row, it.n0 + c + v * 8, a.nk, live);
+        for (int u = 0; u < 4; ++u)
+          q[u] = load_piece<T, VEC>(rows + 8 * u * a.ts, it.n0 + c + (lane & 3) * N, a.nk, live[u]);
       };
       fetch(c0);
       if (BACKWARD && t < a.ntok)
         for (int c = 0; c < a.partials; ++c) s += a.token_s[static_cast<int64_t>(c) * a.ntok + t];
-      T* out = BACKWARD ? static_cast<T*>(a.dlogits) + (t * 2 + it.h) * a.nk : nullptr;
       ok = wait(tfull_bar(acc), (round >> 1) & 1u);
       if (!ok) break;
       ptx::tc_fence_after();
       const uint32_t taddr = tmem + acc * kChunk + (static_cast<uint32_t>(quarter * 32) << 16);
-      for (int c = c0; c < c1; c += 32) {
-        float p[4][8];
+      for (int c = c0; c < c1; c += kColumns) {
 #pragma unroll
-        for (int v = 0; v < 4; ++v) x[v].get(p[v]);
-        if (c + 32 < c1) fetch(c + 32);
-        uint32_t r[32];
-        ptx::tmem_ld_32x32(taddr + c, r);
-        ptx::tmem_ld_wait(r);
+        for (int u = 0; u < 4; ++u) turn[((lane >> 2) + 8 * u) * 5 + (lane & 3)] = q[u];
+        __syncwarp();
+        if (c + kColumns < c1) fetch(c + kColumns);
+        uint32_t r[kColumns];
+        if constexpr (kColumns == 32) {
+          ptx::tmem_ld_32x32(taddr + c, r);
+        } else {
+          ptx::tmem_ld_32x16(taddr + c, r);
+        }
+        float p[4][N];
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const int col = it.n0 + c + v * 8;
+          unpack16<T>(turn[lane * 5 + v], p[v]);
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const float g = __uint_as_float(r[v * 8 + k]);
-            const float e = exp_below(p[v][k] - top);
-            if (BACKWARD) p[v][k] = e * fmaf(g, unscale, -s) * weight;
-            else s = fmaf(e, g, s);
+          for (int k = 0; k < N; ++k) p[v][k] = exp_below(p[v][k] - top);
+        }
+        if constexpr (kColumns == 32) {
+          ptx::tmem_ld_wait(r);
+        } else {
+          ptx::tmem_ld_wait(r);
+        }
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const float g = __uint_as_float(r[v * N + k]);
+            if (BACKWARD) p[v][k] = p[v][k] * fmaf(g, unscale, -s) * weight;
+            else s = fmaf(p[v][k], g, s);
           }
-          if (BACKWARD && t < a.ntok) {
-            if constexpr (VEC) {
-              constexpr int V = Vec16<T>::N;
+          if (BACKWARD) turn[lane * 5 + v] = pack16<T>(p[v]);  // the lane's own row: nobody else reads it before the barrier
+        }
+        __syncwarp();
+        if (BACKWARD) {
 #pragma unroll
-              for (int k = 0; k < 8; k += V)
-                if (col + k < a.nk) *reinterpret_cast<uint4*>(out + col + k) = pack16<T>(*reinterpret_cast<float (*)[V]>(&p[v][k]));
-            } else {
-#pragma unroll
-              for (int k = 0; k < 8; ++k)
-                if (col + k < a.nk) out[col + k] = from_f32<T>(p[v][k]);
-            }
-          }
+          for (int u = 0; u < 4; ++u)
+            if (first + 8 * u < a.ntok)
+              store_piece<T, VEC>(outs + static_cast<int64_t>(16 * u) * a.nk, it.n0 + c + (lane & 3) * N, a.nk,
+                                  turn[((lane >> 2) + 8 * u) * 5 + (lane & 3)]);
+          __syncwarp();
         }
       }
       ptx::tc_fence_before();
@@ -578,7 +659,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
       float top[kRows], inv[kRows];
     };
     Rows now, next;
-    Logits<T, VEC> x[kRows];
+    constexpr int N = Vec16<T>::N, kLoads = 8 / N;
+    uint4 x[kRows][kLoads];
     auto tokens = [&](int i, Rows& w) {
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
@@ -597,7 +679,10 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         const int64_t t = it.t0 + r0 + r * (kMakers * 4);
-        x[r].load(static_cast<const T*>(a.logits) + t * a.ts + (1 - it.h) * a.hs, kb * 64 + piece * 8, a.nk, w.inv[r] != 0.f);
+#pragma unroll
+        for (int k = 0; k < kLoads; ++k)
+          x[r][k] = load_piece<T, VEC>(static_cast<const T*>(a.logits) + t * a.ts + (1 - it.h) * a.hs, kb * 64 + piece * 8 + k * N, a.nk,
+                                       w.inv[r] != 0.f);
       }
     };
     tokens(blockIdx.x, now);
@@ -609,7 +694,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
         float p[kRows][8];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
-          x[r].get(p[r]);
+#pragma unroll
+          for (int k = 0; k < kLoads; ++k) unpack16<T>(x[r][k], *reinterpret_cast<float (*)[N]>(&p[r][k * N]));
 #pragma unroll
           for (int k = 0; k < 8; ++k) p[r][k] = exp_below(p[r][k] - now.top[r]) * (now.inv[r] * 32768.f);
         }
@@ -697,7 +783,7 @@ template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStrea
   const int stage = 2 * kPieceBytes + 2 * a.width * 128;
   a.stages = 200 * 1024 / stage;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  const int smem = a.stages * stage + 1024;
+  const int smem = a.stages * stage + kReaders * kTurnPieces * 16 + 1024;
   const int64_t items = token_tiles(a.ntok) * a.chunks * (BACKWARD ? 2 : 1);
   if (items > 0x7FFFFFFF / kReaders - 65536) return FMOE_ERR_UNSUPPORTED;
   a.items = static_cast<int>(items);
@@ -712,9 +798,13 @@ template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStrea
 
 template <typename T>
 int forward_typed(ProductArgs a, const uint8_t* mask, const int64_t* counts, Prepared* head, float4* stats, Part* part, cudaStream_t stream) {
-  const int64_t want = (a.ntok + 15) / 16, cap = static_cast<int64_t>(device_sm_count()) * 8;
+  const int64_t want = (a.ntok + 31) / 32, cap = static_cast<int64_t>(device_sm_count()) * 8;
   const int64_t grid = want > cap ? cap : want < kParts ? kParts : want;
-  auto* kern = vector_rows<T>(a) ? balance_stats_kernel<T, true> : balance_stats_kernel<T, false>;
+  constexpr int kLine = 8 * Vec16<T>::N;  // columns of eight lanes' pieces
+  auto* kern = !vector_rows<T>(a) ? (a.nk <= 2 * kLine ? balance_stats_kernel<T, false, 2> : balance_stats_kernel<T, false, 4>)
+               : a.nk <= kLine    ? balance_stats_kernel<T, true, 1>
+               : a.nk <= 2 * kLine ? balance_stats_kernel<T, true, 2>
+                                   : balance_stats_kernel<T, true, 4>;
   kern<<<static_cast<unsigned>(grid), 256, 0, stream>>>(static_cast<const T*>(a.logits), a.ts, a.hs, mask, a.ntok, a.nk, stats, counts, part);
   FMOE_LAUNCH_CHECK();
   const int64_t pieces = static_cast<int64_t>(a.padded) * a.padded / 4;
@@ -723,6 +813,50 @@ int forward_typed(ProductArgs a, const uint8_t* mask, const int64_t* counts, Pre
   return launch_product<T, false>(a, stream);
 }
 
+}  // namespace
+
+namespace {
+// Clusters of the histogram that the device runs at once (its GPCs have SMs left over: 15 of 18 on this one); cached per device.
+int histogram_clusters() {
+  static int cache[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (cache[dev] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(device_sm_count() / kHistCtas * kHistCtas);
+    cfg.blockDim = dim3(kHistThreads);
+    cfg.dynamicSmemBytes = kHistExperts * 2;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = kHistCtas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (allow_smem(expert_histogram_kernel, kHistExperts * 2) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, expert_histogram_kernel, &cfg) != cudaSuccess)
+      return 0;
+    cache[dev] = n;
+  }
+  return cache[dev];
+}
+
+template <typename... KArgs, typename... Args>
+int launch_cluster(void (*kern)(KArgs...), int ctas, int threads, int width, int smem, cudaStream_t stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(ctas);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = width;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  FMOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...));
+  return FMOE_OK;
+}
 }  // namespace
 
 int launch_expert_counts(const int64_t* indices, const uint8_t* mask, int64_t T, int k, int64_t N, int64_t* counts, int32_t* status,
@@ -738,20 +872,16 @@ int launch_expert_counts(const int64_t* indices, const uint8_t* mask, int64_t T,
   const int64_t pairs = T * k;
   if (pairs <= 32768 && N <= 131072) {
     const int ctas = pairs <= 4096 && N <= 16384 ? 4 : 8;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(ctas);
-    cfg.blockDim = dim3(kCountThreads);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ctas;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    FMOE_CUDA_TRY(cudaLaunchKernelEx(&cfg, expert_counts_kernel<true>, indices, mask, pairs, k, N, out, status));
-    return FMOE_OK;
+    return launch_cluster(expert_counts_kernel<true>, ctas, kCountThreads, ctas, 0, stream, indices, mask, pairs, k, N, out, status);
   }
   FMOE_CUDA_TRY(cudaMemsetAsync(counts, 0, static_cast<size_t>(N) * 8, stream));
+  if (pairs >= (1 << 20) && N <= kHistExperts && pairs >= 16 * N) {
+    const int smem = static_cast<int>((N + 7) / 8) * 16;
+    const int clusters = histogram_clusters();
+    if (clusters <= 0) return FMOE_ERR_UNSUPPORTED;
+    return launch_cluster(expert_histogram_kernel, clusters * kHistCtas, kHistThreads, kHistCtas, smem, stream, indices, mask, pairs, k,
+                          static_cast<int>(N), out, status);
+  }
   const int64_t want = (pairs + 4 * kCountThreads - 1) / (4 * kCountThreads), cap = device_sm_count();
   expert_counts_kernel<false><<<static_cast<unsigned>(want < cap ? want : cap), kCountThreads, 0, stream>>>(indices, mask, pairs, k, N, out, status);
   FMOE_LAUNCH_CHECK();

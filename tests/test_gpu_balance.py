@@ -39,7 +39,8 @@ def counts_by_hand(indices, N, mask=None):
 
 
 @pytest.mark.parametrize("T,N,k", [(1, 1, 1), (1, 64, 8), (64, 65536, 32), (1000, 100, 7), (4096, 16384, 64), (3, 5, 3),
-                                   (777, 1 << 20, 5), (20000, 16, 4)])
+                                   (777, 1 << 20, 5), (20000, 16, 4), (5000, 60, 64), (70000, 9001, 8), (300000, 16384, 40),
+                                   (9000, 102401, 50)])
 def test_counts(T, N, k):
     from flash_moe_b200 import check_status, expert_counts
 
@@ -59,9 +60,10 @@ def test_counts_of_one_expert():
     """Every selection is the same expert: as many additions to one place as there are."""
     from flash_moe_b200 import expert_counts
 
-    idx = torch.full((5000, 64), 77, device="cuda")
-    got = expert_counts(idx, 16384)
-    assert int(got[77]) == 320000 and int(got.sum()) == 320000
+    for T, k in ((5000, 64), (300, 8), (200000, 64)):
+        for N in (16384, 200000):
+            got = expert_counts(torch.full((T, k), 77, device="cuda"), N)
+            assert int(got[77]) == T * k and int(got.sum()) == T * k
 
 
 def test_counts_leave_bad_ids_out_and_say_so():
