@@ -229,7 +229,7 @@ template <typename T, bool VEC> __device__ __forceinline__ void store_piece(T* r
 // Eight lanes share a row, so a warp has four tokens at a time and a lane enough values for its part of the reductions.  HELD: the
 // 16-byte pieces that a lane holds of each half; what longer rows have beside them is read again for the sum.
 template <typename T, bool VEC, int HELD>
-__global__ void __launch_bounds__(256) balance_stats_kernel(const T* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok,
+__global__ void __launch_bounds__(256, 4) balance_stats_kernel(const T* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok,
                                                             int nk, float4* stats, const int64_t* counts, Part* part) {
   pdl_launch_dependents();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -270,15 +270,18 @@ __global__ void __launch_bounds__(256) balance_stats_kernel(const T* logits, int
   constexpr int N = Vec16<T>::N;
   const int sub = lane & 7;
   const int64_t step = static_cast<int64_t>(gridDim.x) * 32;
+  auto reads = [&](int64_t t) { return t < ntok && (mask == nullptr || mask[t] != 0); };
+  bool ahead = reads((static_cast<int64_t>(blockIdx.x) * 8 + warp) * 4 + (lane >> 3));
   for (int64_t t0 = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * 4; t0 < ntok; t0 += step) {
     const int64_t t = t0 + (lane >> 3);
-    const bool live = t < ntok && (mask == nullptr || mask[t] != 0);
+    const bool live = ahead;
     const T* row[2] = {logits + t * ts, logits + t * ts + hs};
     uint4 q[2][HELD];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int u = 0; u < HELD; ++u) q[h][u] = load_piece<T, VEC>(row[h], (u * 8 + sub) * N, nk, live);
+    ahead = reads(t + step);
     float top[2], sum[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -406,6 +409,18 @@ constexpr int kPieceBytes = kTileTokens * 128;  // one piece of the probabilitie
 constexpr int kMaxStages = 4;
 constexpr int kTurnPieces = 32 * 5;  // shared memory of a reading warp, in 16-byte pieces
 
+// a stage of the ring and the parity of its use
+struct RingCursor {
+  int stage = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++stage == stages) {
+      stage = 0;
+      parity ^= 1u;
+    }
+  }
+};
+
 struct ProductArgs {
   const void* logits;
   int64_t ts, hs, ntok;
@@ -497,13 +512,14 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
   if (warp == 0) {
     bool ok = true;
     uint32_t use = 0;  // stages used so far
+    RingCursor ring;
     for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x) {
       const Item it = item_of(i);
       const int64_t per = static_cast<int64_t>(a.padded) * a.padded / 8;
       const uint32_t bytes = static_cast<uint32_t>(it.columns) * 128u;
-      for (int kb = 0; kb < blocks; ++kb, ++use) {
-        const int s = use % a.stages;
-        ok = wait(empty_bar(s), ((use / a.stages) & 1u) ^ 1u);
+      for (int kb = 0; kb < blocks; ++kb, ++use, ring.next(a.stages)) {
+        const int s = ring.stage;
+        ok = wait(empty_bar(s), ring.parity ^ 1u);
         if (!ok) break;
         if (ptx::elect_one()) {
           const uint4* src = a.pieces + 2 * it.h * per + (static_cast<int64_t>(kb) * a.padded + it.n0) * 8;
@@ -521,16 +537,17 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
     }
   } else if (warp == 1) {
     bool ok = true;
-    uint32_t use = 0, round = 0;
+    uint32_t round = 0;
+    RingCursor ring;
     for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x, ++round) {
       const Item it = item_of(i);
       const uint32_t acc = round & 1u;
       ok = wait(tempty_bar(acc), ((round >> 1) & 1u) ^ 1u);
       // float16 operands, float32 accumulator, 128 rows
       const uint32_t idesc = (1u << 4) | (static_cast<uint32_t>(it.columns >> 3) << 17) | (8u << 24);
-      for (int kb = 0; kb < blocks && ok; ++kb, ++use) {
-        const int s = use % a.stages;
-        ok = wait(full_bar(s), (use / a.stages) & 1u) && wait(ready_bar(s), (use / a.stages) & 1u);
+      for (int kb = 0; kb < blocks && ok; ++kb, ring.next(a.stages)) {
+        const int s = ring.stage;
+        ok = wait(full_bar(s), ring.parity) && wait(ready_bar(s), ring.parity);
         if (!ok) break;
         ptx::tc_fence_after();
         const uint32_t st = base + s * stage_bytes;
@@ -560,6 +577,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
     // thread per row would touch 32.  The chunk changes hands in shared memory, rows 80 bytes apart.
     constexpr int N = Vec16<T>::N, kColumns = 4 * N;
     uint4* turn = reinterpret_cast<uint4*>(gen + a.stages * stage_bytes) + (warp - 2) * kTurnPieces;
+    const int64_t stride = 8 * a.ts, out_stride = 16 * static_cast<int64_t>(a.nk);
     const float unscale = a.head->unscale;
     const float scale = BACKWARD ? static_cast<float>(a.head->coef * static_cast<double>(*a.upstream)) : 0.f;
     for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x, ++round) {
@@ -576,16 +594,18 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
       const float weight = BACKWARD ? (inv != 0.f ? inv * scale : 0.f) : inv * unscale;
       // the lane's part of a chunk in memory: piece lane % 4 of the rows lane / 4 + 8 u
       const int64_t first = it.t0 + quarter * 32 + (lane >> 2);
-      const T* rows = static_cast<const T*>(a.logits) + first * a.ts + it.h * a.hs;
-      T* outs = BACKWARD ? static_cast<T*>(a.dlogits) + (first * 2 + it.h) * a.nk : nullptr;
+      const int ahead = it.n0 + (lane & 3) * N;
+      const T* rows = static_cast<const T*>(a.logits) + first * a.ts + it.h * a.hs + ahead;
+      T* outs = BACKWARD ? static_cast<T*>(a.dlogits) + (first * 2 + it.h) * a.nk + ahead : nullptr;
+      const int left = a.nk - ahead;  // columns from the lane's piece of the first chunk to the row's end
       bool live[4];
 #pragma unroll
       for (int u = 0; u < 4; ++u) live[u] = __shfl_sync(kFull, inv, (lane >> 2) + 8 * u) != 0.f;
       uint4 q[4];
       auto fetch = [&](int c) {
+        const T* at = rows + c;
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
-          q[u] = load_piece<T, VEC>(rows + 8 * u * a.ts, it.n0 + c + (lane & 3) * N, a.nk, live[u]);
+        for (int u = 0; u < 4; ++u, at += stride) q[u] = load_piece<T, VEC>(at, 0, left - c, live[u]);
       };
       fetch(c0);
       if (BACKWARD && t < a.ntok)
@@ -629,11 +649,10 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
         }
         __syncwarp();
         if (BACKWARD) {
+          T* out = outs + c;
 #pragma unroll
-          for (int u = 0; u < 4; ++u)
-            if (first + 8 * u < a.ntok)
-              store_piece<T, VEC>(outs + static_cast<int64_t>(16 * u) * a.nk, it.n0 + c + (lane & 3) * N, a.nk,
-                                  turn[((lane >> 2) + 8 * u) * 5 + (lane & 3)]);
+          for (int u = 0; u < 4; ++u, out += out_stride)
+            if (first + 8 * u < a.ntok) store_piece<T, VEC>(out, 0, left - c, turn[((lane >> 2) + 8 * u) * 5 + (lane & 3)]);
           __syncwarp();
         }
       }
@@ -650,60 +669,60 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
     }
   } else {
     bool ok = true;
-    uint32_t use = 0;
+    RingCursor ring;
     // thread -> rows r0, r0 + 32, ... and a fixed 16-byte place (8 columns) of each 64-column block
     const int id = threadIdx.x - (2 + kReaders) * 32, piece = id & 7, r0 = id >> 3;
     const int place = piece ^ (r0 & 7);
-    constexpr int kRows = kTileTokens / (kMakers * 4);
+    constexpr int kStep = kMakers * 4, kRows = kTileTokens / kStep;
+    constexpr int N = Vec16<T>::N, kLoads = 8 / N;
     struct Rows {
+      const T* first;  // the thread's first row, at its place of the first block
       float top[kRows], inv[kRows];
     };
     Rows now, next;
-    constexpr int N = Vec16<T>::N, kLoads = 8 / N;
     uint4 x[kRows][kLoads];
     auto tokens = [&](int i, Rows& w) {
+      const Item it = item_of(i);
+      const int64_t t0 = it.t0 + r0;
+      w.first = static_cast<const T*>(a.logits) + t0 * a.ts + (1 - it.h) * a.hs + piece * 8;
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
-        const Item it = item_of(i);
-        const int64_t t = it.t0 + r0 + r * (kMakers * 4);
         w.top[r] = w.inv[r] = 0.f;
-        if (i < a.items && t < a.ntok) {
-          const float4 st = a.stats[t];
+        if (i < a.items && t0 + r * kStep < a.ntok) {
+          const float4 st = a.stats[t0 + r * kStep];
           w.top[r] = it.h == 0 ? st.z : st.x;
           w.inv[r] = it.h == 0 ? st.w : st.y;
         }
       }
     };
-    auto fetch = [&](int i, int kb, const Rows& w) {
-      const Item it = item_of(i);
+    const int64_t stride = kStep * a.ts;
+    auto fetch = [&](int kb, const Rows& w) {
+      const T* at = w.first + kb * 64;
+      const int left = a.nk - kb * 64 - piece * 8;  // columns from here to the row's end
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const int64_t t = it.t0 + r0 + r * (kMakers * 4);
+      for (int r = 0; r < kRows; ++r, at += stride)
 #pragma unroll
-        for (int k = 0; k < kLoads; ++k)
-          x[r][k] = load_piece<T, VEC>(static_cast<const T*>(a.logits) + t * a.ts + (1 - it.h) * a.hs, kb * 64 + piece * 8 + k * N, a.nk,
-                                       w.inv[r] != 0.f);
-      }
+        for (int k = 0; k < kLoads; ++k) x[r][k] = load_piece<T, VEC>(at, k * N, left, w.inv[r] != 0.f);
     };
     tokens(blockIdx.x, now);
-    fetch(blockIdx.x, 0, now);
+    fetch(0, now);
     for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x) {
       tokens(i + gridDim.x, next);
-      for (int kb = 0; kb < blocks; ++kb, ++use) {
-        const int s = use % a.stages;
+      for (int kb = 0; kb < blocks; ++kb, ring.next(a.stages)) {
         float p[kRows][8];
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
+          const float weight = now.inv[r] * 32768.f;
 #pragma unroll
           for (int k = 0; k < kLoads; ++k) unpack16<T>(x[r][k], *reinterpret_cast<float (*)[N]>(&p[r][k * N]));
 #pragma unroll
-          for (int k = 0; k < 8; ++k) p[r][k] = exp_below(p[r][k] - now.top[r]) * (now.inv[r] * 32768.f);
+          for (int k = 0; k < 8; ++k) p[r][k] = exp_below(p[r][k] - now.top[r]) * weight;
         }
-        if (kb + 1 < blocks) fetch(i, kb + 1, now);
-        else fetch(i + gridDim.x, 0, next);
-        ok = wait(empty_bar(s), ((use / a.stages) & 1u) ^ 1u);
+        if (kb + 1 < blocks) fetch(kb + 1, now);
+        else fetch(0, next);
+        ok = wait(empty_bar(ring.stage), ring.parity ^ 1u);
         if (!ok) break;
-        uint4* dst = reinterpret_cast<uint4*>(gen + s * stage_bytes);
+        uint4* dst = reinterpret_cast<uint4*>(gen + ring.stage * stage_bytes) + r0 * 8 + place;
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
           uint32_t hi[4], lo[4];
@@ -715,13 +734,12 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
             hi[k] = *reinterpret_cast<const uint32_t*>(&h);
             lo[k] = *reinterpret_cast<const uint32_t*>(&l);
           }
-          const int at = (r0 + r * (kMakers * 4)) * 8 + place;
-          dst[at] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
-          dst[at + kPieceBytes / 16] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+          dst[r * kStep * 8] = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+          dst[r * kStep * 8 + kPieceBytes / 16] = make_uint4(lo[0], lo[1], lo[2], lo[3]);
         }
         ptx::fence_async_smem();
         __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(ready_bar(s));
+        if (lane == 0) ptx::mbar_arrive(ready_bar(ring.stage));
       }
       now = next;
     }
@@ -798,7 +816,7 @@ template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStrea
 
 template <typename T>
 int forward_typed(ProductArgs a, const uint8_t* mask, const int64_t* counts, Prepared* head, float4* stats, Part* part, cudaStream_t stream) {
-  const int64_t want = (a.ntok + 31) / 32, cap = static_cast<int64_t>(device_sm_count()) * 8;
+  const int64_t want = (a.ntok + 31) / 32, cap = static_cast<int64_t>(device_sm_count()) * 16;
   const int64_t grid = want > cap ? cap : want < kParts ? kParts : want;
   constexpr int kLine = 8 * Vec16<T>::N;  // columns of eight lanes' pieces
   auto* kern = !vector_rows<T>(a) ? (a.nk <= 2 * kLine ? balance_stats_kernel<T, false, 2> : balance_stats_kernel<T, false, 4>)
