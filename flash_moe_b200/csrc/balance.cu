@@ -196,6 +196,22 @@ template <typename T> __device__ __forceinline__ uint32_t minus_infinity() { ret
 template <> __device__ __forceinline__ uint32_t minus_infinity<__nv_bfloat16>() { return 0xFF80FF80u; }
 template <> __device__ __forceinline__ uint32_t minus_infinity<__half>() { return 0xFC00FC00u; }
 
+// the larger of each pair of values of two pieces; the other one where one is a NaN
+template <typename T> __device__ __forceinline__ uint4 piece_max(const uint4& a, const uint4& b) {
+  uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) {
+      x[i] = __float_as_uint(fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
+    } else {
+      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+      const T2 m = __hmax2(*reinterpret_cast<const T2*>(&x[i]), *reinterpret_cast<const T2*>(&y[i]));
+      x[i] = *reinterpret_cast<const uint32_t*>(&m);
+    }
+  }
+  return make_uint4(x[0], x[1], x[2], x[3]);
+}
+
 // Pieces of a row: 16 bytes, 8 or 4 logits, from column c on.  What lies behind the row's end, or in a row that is not read, is
 // minus infinity: its exponential is 0 and no use of the values has to ask.  VEC: rows are made of aligned pieces.
 template <typename T, bool VEC> __device__ __forceinline__ uint4 load_piece(const T* row, int c, int nk, bool read = true) {
@@ -285,17 +301,16 @@ __global__ void __launch_bounds__(256, 4) balance_stats_kernel(const T* logits, 
     float top[2], sum[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      top[h] = -INFINITY;
-      auto join = [&](const uint4& v) {
-        float f[N];
-        unpack16<T>(v, f);
+      uint4 m = q[h][0];
 #pragma unroll
-        for (int i = 0; i < N; ++i) top[h] = fmaxf(top[h], f[i]);
-      };
-#pragma unroll
-      for (int u = 0; u < HELD; ++u) join(q[h][u]);
+      for (int u = 1; u < HELD; ++u) m = piece_max<T>(m, q[h][u]);
       if (live)
-        for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) join(load_piece<T, VEC>(row[h], c, nk));
+        for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) m = piece_max<T>(m, load_piece<T, VEC>(row[h], c, nk));
+      float f[N];
+      unpack16<T>(m, f);
+      top[h] = f[0];
+#pragma unroll
+      for (int i = 1; i < N; ++i) top[h] = fmaxf(top[h], f[i]);
     }
 #pragma unroll
     for (int d = 4; d > 0; d >>= 1) {
@@ -304,17 +319,18 @@ __global__ void __launch_bounds__(256, 4) balance_stats_kernel(const T* logits, 
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      sum[h] = 0.f;
+      float part[4] = {0.f, 0.f, 0.f, 0.f};
       auto join = [&](const uint4& v) {
         float f[N];
         unpack16<T>(v, f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[h] += exp_below(f[i] - top[h]);
+        for (int i = 0; i < N; ++i) part[i & 3] += exp_below(f[i] - top[h]);
       };
 #pragma unroll
       for (int u = 0; u < HELD; ++u) join(q[h][u]);
       if (live)
         for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) join(load_piece<T, VEC>(row[h], c, nk));
+      sum[h] = (part[0] + part[1]) + (part[2] + part[3]);
     }
 #pragma unroll
     for (int d = 4; d > 0; d >>= 1) {
