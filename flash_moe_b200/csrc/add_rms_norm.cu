@@ -102,7 +102,8 @@ template <typename T> struct NormArgs {
   __nv_fp8_storage_t* q;
   float* scales;
   int64_t rows;
-  int H, pieces, batch, group, groups;
+  int H, pieces, batch;
+  int group_shift, groups;  // kFp8Block: columns of a block, a power of two
   float eps;
 };
 
@@ -214,9 +215,28 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_kernel(const No
         const int p = c * NT + tid;
         if (!live(0, p)) continue;
         value(0, c, y);
-        atomicMax(m + p / a.group, __float_as_uint(fabsf(y[0])));
+        atomicMax(m + (p >> a.group_shift), __float_as_uint(fabsf(y[0])));
       }
       group_barrier<WPG>();
+    }
+    float most[R][C];
+    if (MODE == kFp8Block && VEC > 1) {
+      // a block is 4 to 32 neighbouring lanes
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          float y[VEC];
+          value(r, c, y);
+          most[r][c] = 0.f;
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) most[r][c] = MaxOp::join(most[r][c], fabsf(y[i]));
+        }
+      for (int d = (1 << a.group_shift) / (2 * VEC); d > 0; d >>= 1)
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+          for (int c = 0; c < C; ++c) most[r][c] = MaxOp::join(most[r][c], __shfl_xor_sync(kFull, most[r][c], d));
     }
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -224,28 +244,21 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_kernel(const No
       for (int c = 0; c < C; ++c) {
         const int p = c * NT + tid;
         const bool ok = live(r, p);
-        float y[VEC], m = 0.f;
+        float y[VEC], m;
         value(r, c, y);
-        const int64_t col = static_cast<int64_t>(p) * VEC;
+        const int col = p * VEC;
         if (MODE == kFp8Row) m = top[r];
-        else if (VEC == 1) m = ok ? __uint_as_float(block_max[g * a.groups + p / a.group]) : 0.f;
-        else {
-          // a block is a.group / VEC neighbouring lanes, 4 to 32 of them
-          if (ok) {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) m = MaxOp::join(m, fabsf(y[i]));
-          }
-          m = warp_join<MaxOp>(m, a.group / VEC);
-        }
+        else if (VEC == 1) m = ok ? __uint_as_float(block_max[g * a.groups + (p >> a.group_shift)]) : 0.f;
+        else m = most[r][c];
         if (!ok) continue;
-        m = m / kE4m3Max;
+        m *= 1.f / kE4m3Max;
         const float scale = m < kMinScale ? kMinScale : m;  // a NaN stays
-        const float inv = 1.f / scale;
+        const float inv = __fdividef(1.f, scale);           // 2^-126 <= scale < 2^120, or infinite: 0
         const int64_t at = (r0 + r) * a.H + col;
         if (MODE == kFp8Row) {
           if (p == 0) a.scales[r0 + r] = scale;
-        } else if (col % a.group == 0) {
-          a.scales[(r0 + r) * a.groups + col / a.group] = scale;
+        } else if ((col & ((1 << a.group_shift) - 1)) == 0) {
+          a.scales[(r0 + r) * a.groups + (col >> a.group_shift)] = scale;
         }
         if (a.residual != nullptr) s[r][c].store(a.summed + at);
         if (VEC == 1) {
@@ -298,23 +311,33 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_backward_kernel
   int turn = 0;
   const int64_t slot = static_cast<int64_t>(blockIdx.x) * Group<WPG>::kPerCta + g;
   const int64_t step = static_cast<int64_t>(gridDim.x) * Group<WPG>::kPerCta * a.batch;
-  for (int64_t r0 = slot * a.batch; r0 < a.rows; r0 += step, turn ^= 1) {
+  struct Batch {
     Piece<T, VEC> s[R][C], dn[R][C], ds[R][C];
+  };
+  auto fetch = [&](int64_t r0, Batch& b) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int p = c * NT + tid;
-        s[r][c].zero();
-        dn[r][c].zero();
-        ds[r][c].zero();
+        b.s[r][c].zero();
+        b.dn[r][c].zero();
+        b.ds[r][c].zero();
         if (r < a.batch && r0 + r < a.rows && p < a.pieces) {
           const int64_t at = (r0 + r) * a.H + static_cast<int64_t>(p) * VEC;
-          s[r][c].load(a.summed + at);
-          dn[r][c].load(a.dnormed + at);
-          if (a.dsummed != nullptr) ds[r][c].load(a.dsummed + at);
+          b.s[r][c].load(a.summed + at);
+          b.dn[r][c].load(a.dnormed + at);
+          if (a.dsummed != nullptr) b.ds[r][c].load(a.dsummed + at);
         }
       }
+  };
+  Batch now, next;
+  if (slot * a.batch < a.rows) fetch(slot * a.batch, now);
+  for (int64_t r0 = slot * a.batch; r0 < a.rows; r0 += step, turn ^= 1) {
+    if (r0 + step < a.rows) fetch(r0 + step, next);  // on the way while this batch is worked on
+    auto& s = now.s;
+    auto& dn = now.dn;
+    auto& ds = now.ds;
     float sum[2 * R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -359,6 +382,7 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_backward_kernel
         out.store(a.dx + (r0 + r) * a.H + static_cast<int64_t>(p) * VEC);
       }
     }
+    now = next;
   }
   if (a.part != nullptr) {
 #pragma unroll
@@ -390,12 +414,18 @@ __global__ void __launch_bounds__(256) rms_norm_dweight_kernel(const float* part
 
 constexpr int kMaxHidden = 16384;
 
-// The shape of a call: how many warps share a row and how many pieces a thread holds of it
+// The shape of a call: how many warps share a row, how many pieces a thread holds of it, and how many rows at a time forward and
+// backward take.  Few warps with two pieces a thread beat many with one: less of a row's time goes into reductions across warps.
 struct Shape {
-  int wpg, c, r;
+  int wpg, c;
 };
-constexpr Shape kVecShapes[] = {{1, 1, 4}, {4, 1, 4}, {8, 1, 4}, {8, 2, 2}, {16, 2, 2}, {32, 4, 1}};
-constexpr Shape kOneShapes[] = {{1, 8, 1}, {8, 8, 1}, {32, 16, 1}};
+#define FMOE_VEC_SHAPES(X) X(0, 1, 1, 4, 2) X(1, 1, 2, 1, 1) X(2, 2, 2, 1, 1) X(3, 4, 2, 1, 1) X(4, 8, 2, 1, 1) X(5, 8, 4, 1, 1) \
+  X(6, 16, 4, 1, 1) X(7, 32, 4, 1, 1)
+#define FMOE_ONE_SHAPES(X) X(0, 1, 8, 1, 1) X(1, 8, 8, 1, 1) X(2, 32, 16, 1, 1)
+#define FMOE_SHAPE(I_, W_, C_, RF_, RB_) {W_, C_},
+constexpr Shape kVecShapes[] = {FMOE_VEC_SHAPES(FMOE_SHAPE)};
+constexpr Shape kOneShapes[] = {FMOE_ONE_SHAPES(FMOE_SHAPE)};
+#undef FMOE_SHAPE
 int shape_of(bool vec, int pieces) {
   int i = 0;
   if (vec) {
@@ -406,10 +436,11 @@ int shape_of(bool vec, int pieces) {
   return i;
 }
 
-// groups that the grid of a backward has, at most
-int64_t backward_groups(int wpg, int64_t rows) {
-  const int cta = wpg < 8 ? 256 : 32 * wpg, per_cta = cta / (32 * wpg);
-  const int64_t cap = static_cast<int64_t>(device_sm_count()) * (cta <= 256 ? 2 : 1) * per_cta;
+// Groups that the grid of a backward has: all that its registers let run at once, and no more, since each group leaves a row of
+// partial sums.
+int64_t backward_groups(Shape sh, int64_t rows) {
+  const int cta = sh.wpg < 8 ? 256 : 32 * sh.wpg, per_cta = cta / (32 * sh.wpg);
+  const int64_t cap = static_cast<int64_t>(device_sm_count()) * (sh.wpg * sh.c <= 16 ? 2 : 1) * per_cta;
   return rows < cap ? (rows + per_cta - 1) / per_cta * per_cta : cap;
 }
 
@@ -440,7 +471,7 @@ int launch_backward(const NormBackwardArgs<T>& in, T* dweight, cudaStream_t stre
   NormBackwardArgs<T> a = in;
   constexpr int per_cta = Group<WPG>::kPerCta;
   a.batch = batch_rows(a.rows, R, per_cta);
-  const int64_t groups = backward_groups(WPG, a.rows);
+  const int64_t groups = backward_groups({WPG, C}, a.rows);
   add_rms_norm_backward_kernel<T, VEC, WPG, C, R><<<static_cast<unsigned>(groups / per_cta), Group<WPG>::kCta, 0, stream>>>(a);
   FMOE_LAUNCH_CHECK();
   if (dweight != nullptr) {
@@ -450,24 +481,6 @@ int launch_backward(const NormBackwardArgs<T>& in, T* dweight, cudaStream_t stre
   return FMOE_OK;
 }
 
-#define FMOE_NORM_SHAPES(CALL)                          \
-  if (vec) {                                            \
-    constexpr int V = Vec16<T>::N;                      \
-    switch (shape_of(true, a.pieces)) {                 \
-      case 0: return CALL(V, 1, 1, 4);                  \
-      case 1: return CALL(V, 4, 1, 4);                  \
-      case 2: return CALL(V, 8, 1, 4);                  \
-      case 3: return CALL(V, 8, 2, 2);                  \
-      case 4: return CALL(V, 16, 2, 2);                 \
-      default: return CALL(V, 32, 4, 1);                \
-    }                                                   \
-  }                                                     \
-  switch (shape_of(false, a.pieces)) {                  \
-    case 0: return CALL(1, 1, 8, 1);                    \
-    case 1: return CALL(1, 8, 8, 1);                    \
-    default: return CALL(1, 32, 16, 1);                 \
-  }
-
 template <typename T>
 int forward_typed(const void* x, const void* residual, const void* weight, void* summed, void* normed, void* q, float* scales,
                   int64_t rows, int H, int group, float eps, int mode, cudaStream_t stream) {
@@ -475,10 +488,15 @@ int forward_typed(const void* x, const void* residual, const void* weight, void*
                    aligned16(normed) && aligned16(q);
   NormArgs<T> a = {static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight),
                    static_cast<T*>(summed), static_cast<T*>(normed), static_cast<__nv_fp8_storage_t*>(q), scales, rows, H,
-                   vec ? H / Vec16<T>::N : H, 1, group, mode == kFp8Block ? (H + group - 1) / group : 1, eps};
-#define FMOE_CALL(V_, W_, C_, R_) launch_forward<T, V_, W_, C_, R_>(a, mode, stream)
-  FMOE_NORM_SHAPES(FMOE_CALL)
-#undef FMOE_CALL
+                   vec ? H / Vec16<T>::N : H, 1, group == 32 ? 5 : group == 64 ? 6 : 7, mode == kFp8Block ? (H + group - 1) / group : 1, eps};
+  const int shape = shape_of(vec, a.pieces);
+#define FMOE_VEC(I_, W_, C_, RF_, RB_) if (vec && shape == I_) return launch_forward<T, Vec16<T>::N, W_, C_, RF_>(a, mode, stream);
+#define FMOE_ONE(I_, W_, C_, RF_, RB_) if (!vec && shape == I_) return launch_forward<T, 1, W_, C_, RF_>(a, mode, stream);
+  FMOE_VEC_SHAPES(FMOE_VEC)
+  FMOE_ONE_SHAPES(FMOE_ONE)
+#undef FMOE_VEC
+#undef FMOE_ONE
+  return FMOE_ERR_UNSUPPORTED;
 }
 
 bool backward_vec(int dtype, int H, const void* a, const void* b, const void* c, const void* d, const void* e) {
@@ -492,9 +510,14 @@ int backward_typed(const void* dnormed, const void* dsummed, const void* summed,
                            static_cast<const T*>(weight), static_cast<T*>(dx), dweight != nullptr ? part : nullptr, rows, H,
                            vec ? H / Vec16<T>::N : H, 1, eps};
   T* dw = static_cast<T*>(dweight);
-#define FMOE_CALL(V_, W_, C_, R_) launch_backward<T, V_, W_, C_, R_>(a, dw, stream)
-  FMOE_NORM_SHAPES(FMOE_CALL)
-#undef FMOE_CALL
+  const int shape = shape_of(vec, a.pieces);
+#define FMOE_VEC(I_, W_, C_, RF_, RB_) if (vec && shape == I_) return launch_backward<T, Vec16<T>::N, W_, C_, RB_>(a, dw, stream);
+#define FMOE_ONE(I_, W_, C_, RF_, RB_) if (!vec && shape == I_) return launch_backward<T, 1, W_, C_, RB_>(a, dw, stream);
+  FMOE_VEC_SHAPES(FMOE_VEC)
+  FMOE_ONE_SHAPES(FMOE_ONE)
+#undef FMOE_VEC
+#undef FMOE_ONE
+  return FMOE_ERR_UNSUPPORTED;
 }
 
 }  // namespace
@@ -521,9 +544,9 @@ int launch_add_rms_norm(const void* x, const void* residual, const void* weight,
 size_t add_rms_norm_backward_workspace_bytes(int64_t rows, int H, int dtype) {
   if (rows <= 0 || H <= 0 || H > kMaxHidden) return 0;
   const int n = 16 / dtype_size(dtype);
-  int64_t groups = backward_groups(kOneShapes[shape_of(false, H)].wpg, rows);
+  int64_t groups = backward_groups(kOneShapes[shape_of(false, H)], rows);
   if (H % n == 0) {
-    const int64_t v = backward_groups(kVecShapes[shape_of(true, H / n)].wpg, rows);
+    const int64_t v = backward_groups(kVecShapes[shape_of(true, H / n)], rows);
     groups = v > groups ? v : groups;
   }
   return static_cast<size_t>(groups) * H * sizeof(float);
