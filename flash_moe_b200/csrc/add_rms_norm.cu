@@ -8,6 +8,9 @@
 // stored and the backward finds the same s; n, dx and dw are rounded once.
 #include <cuda_fp8.h>
 
+#include <cstring>
+#include <initializer_list>
+
 #include "common.cuh"
 
 namespace fmoe {
@@ -47,6 +50,104 @@ template <int WPG> __device__ __forceinline__ void group_barrier() {
   else if (Group<WPG>::kPerCta == 1) __syncthreads();
   else asm volatile("bar.sync %0, %1;" ::"r"(static_cast<int>(threadIdx.x) / Group<WPG>::kThreads + 1), "n"(Group<WPG>::kThreads) : "memory");
 }
+
+// Values lo to hi - 1 of a piece, those that lie in its row.  Only a row's ends come here.
+template <typename T, int VEC> __device__ __forceinline__ void load_part(Piece<T, VEC>& piece, const T* at, int lo, int hi) {
+  T v[VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) v[i] = i >= lo && i < hi ? at[i] : from_f32<T>(0.f);
+  memcpy(&piece, v, sizeof(v));
+}
+// LOOP: unrolled, the stores take registers that a kernel with little else to hold gives to another CTA (32768 rows of 1001
+// bfloat16: 60 us instead of 90); the 8-bit kernels are faster with them unrolled (106 us instead of 114).
+template <bool LOOP, typename T, int VEC> __device__ __forceinline__ void store_part(const Piece<T, VEC>& piece, T* at, int lo, int hi) {
+  if constexpr (VEC == 1) {
+    if (lo < hi) piece.store(at);
+  } else if constexpr (!LOOP) {
+    T v[VEC];
+    memcpy(v, &piece, sizeof(v));
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i >= lo && i < hi) at[i] = v[i];
+  } else {
+    constexpr int kBits = 8 * sizeof(T), kWord = 4 / sizeof(T);
+#pragma unroll 1
+    for (int i = lo; i < hi; ++i) {
+      const int word = i / kWord;
+      const uint32_t w = word == 0 ? piece.q.x : word == 1 ? piece.q.y : word == 2 ? piece.q.z : piece.q.w;
+      const std::conditional_t<sizeof(T) == 2, uint16_t, uint32_t> bits = w >> (i % kWord * kBits % 32);
+      memcpy(at + i, &bits, sizeof(T));
+    }
+  }
+}
+// zero outside [lo, hi)
+template <typename T, int VEC> __device__ __forceinline__ void keep_part(Piece<T, VEC>& piece, int lo, int hi) {
+  if constexpr (VEC > 1) {
+    uint32_t w[4] = {piece.q.x, piece.q.y, piece.q.z, piece.q.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (sizeof(T) == 4) {
+        w[j] = j >= lo && j < hi ? w[j] : 0u;
+      } else {
+        const uint32_t low = 2 * j >= lo && 2 * j < hi ? 0x0000FFFFu : 0u, high = 2 * j + 1 >= lo && 2 * j + 1 < hi ? 0xFFFF0000u : 0u;
+        w[j] &= low | high;
+      }
+    }
+    piece.q = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// How a group walks over rows and a thread over a row's pieces.  Rows whose length is no multiple of a piece start at any value of
+// one, but rows r, r + VEC, r + 2 VEC, ... all at the same: with SHIFT a group takes the rows of one remainder, and its pieces are
+// the aligned ones of memory, of which a row's first and last lie in it in part.  A thread's columns, its weights and its part of
+// dweight are the same for every row then.  Pieces are read whole, with the neighbours' values, which `mask` takes out where they
+// are used (a wait inside the read would stop the reads behind it); only the last row's end is read value by value.
+template <int VEC, int WPG, bool SHIFT> struct Walk {
+  int64_t row, step, rows;
+  int H, shift, pieces;
+  __device__ __forceinline__ Walk(int64_t rows_, int H_, int batch) : rows(rows_), H(H_) {
+    const int64_t group = static_cast<int64_t>(blockIdx.x) * (Group<WPG>::kPerCta) + threadIdx.x / Group<WPG>::kThreads;
+    const int64_t groups = static_cast<int64_t>(gridDim.x) * Group<WPG>::kPerCta;
+    if (SHIFT) {
+      row = group;  // groups is a multiple of VEC: group + j * groups keeps the remainder
+      step = groups;
+      shift = static_cast<int>((group % VEC) * H % VEC);
+    } else {
+      row = group * batch;
+      step = groups * batch;
+      shift = 0;
+    }
+    pieces = (H + shift + VEC - 1) / VEC;
+  }
+  __device__ __forceinline__ int col(int piece) const { return piece * VEC - shift; }
+  __device__ __forceinline__ bool whole(int piece) const {
+    return !SHIFT ? piece < pieces : col(piece) >= 0 && col(piece) + VEC <= H;
+  }
+  // the part of a piece that lies in the row
+  __device__ __forceinline__ int lo(int piece) const { return col(piece) < 0 ? -col(piece) : 0; }
+  __device__ __forceinline__ int hi(int piece) const { return H - col(piece) < VEC ? H - col(piece) : VEC; }
+  // the piece of row r of an array
+  template <typename T> __device__ __forceinline__ void load(Piece<T, VEC>& p, const T* base, int64_t r, int piece) const {
+    if (piece >= pieces) return;
+    const T* at = base + r * H + col(piece);
+    if (!SHIFT || r + 1 < rows || col(piece) + VEC <= H) p.load(at);
+    else load_part<T, VEC>(p, at, lo(piece), hi(piece));
+  }
+  template <typename T> __device__ __forceinline__ void mask(Piece<T, VEC>& p, int piece) const {
+    if (SHIFT && piece < pieces && !whole(piece)) keep_part<T, VEC>(p, lo(piece), hi(piece));
+  }
+  template <bool LOOP = true, typename T> __device__ __forceinline__ void store(const Piece<T, VEC>& p, T* row, int piece) const {
+    if (whole(piece)) p.store(row + col(piece));
+    else if (SHIFT && piece < pieces) store_part<LOOP, T, VEC>(p, row + col(piece), lo(piece), hi(piece));
+  }
+  // weights are not aligned like the rows
+  template <typename T> __device__ __forceinline__ void weights(Piece<T, VEC>& p, const T* w, int piece) const {
+    p.zero();
+    if (w == nullptr || piece >= pieces) return;
+    if (SHIFT) load_part<T, VEC>(p, w + col(piece), lo(piece), hi(piece));
+    else p.load(w + col(piece));
+  }
+};
 
 struct SumOp {
   static __device__ __forceinline__ float zero() { return 0.f; }
@@ -102,42 +203,41 @@ template <typename T> struct NormArgs {
   __nv_fp8_storage_t* q;
   float* scales;
   int64_t rows;
-  int H, pieces, batch;
+  int H, batch;
   int group_shift, groups;  // kFp8Block: columns of a block, a power of two
   float eps;
 };
 
-template <typename T, int VEC, int WPG, int C, int R, int MODE>
-__global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_kernel(const NormArgs<T> a) {
+template <typename T, int VEC, int WPG, int C, int R, bool SHIFT, int MODE>
+__global__ void __launch_bounds__(Group<WPG>::kCta, Group<WPG>::kCta > 256 ? 1 : C > 2 ? 2 : 4)
+add_rms_norm_kernel(const NormArgs<T> a) {
   constexpr int NT = Group<WPG>::kThreads;
+  constexpr bool kTable = MODE == kFp8Block && (VEC == 1 || SHIFT);  // a piece may lie in two blocks, or a block in many warps
   const int g = threadIdx.x / NT, tid = threadIdx.x % NT;
   __shared__ float slots[Group<WPG>::kPerCta][3][R * WPG];
-  extern __shared__ uint32_t block_max[];  // kFp8Block on single values: [kPerCta][groups]
+  extern __shared__ uint32_t block_max[];  // kTable: [kPerCta][groups]
+  const Walk<VEC, WPG, SHIFT> walk(a.rows, a.H, a.batch);
   Piece<T, VEC> w[C];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int p = c * NT + tid;
-    w[c].zero();
-    if (a.weight != nullptr && p < a.pieces) w[c].load(a.weight + static_cast<int64_t>(p) * VEC);
+    walk.weights(w[c], a.weight, c * NT + tid);
   }
   int turn = 0;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * Group<WPG>::kPerCta * a.batch;
-  for (int64_t r0 = (static_cast<int64_t>(blockIdx.x) * Group<WPG>::kPerCta + g) * a.batch; r0 < a.rows; r0 += step, turn ^= 1) {
+  for (int64_t r0 = walk.row; r0 < a.rows; r0 += walk.step, turn ^= 1) {
     Piece<T, VEC> s[R][C];
     float sq[R];
+    auto row_live = [&](int r) { return R == 1 || (r < a.batch && r0 + r < a.rows); };
     {
       Piece<T, VEC> res[R][C];
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const int p = c * NT + tid;
           s[r][c].zero();
           res[r][c].zero();
-          if (r < a.batch && r0 + r < a.rows && p < a.pieces) {
-            const int64_t at = (r0 + r) * a.H + static_cast<int64_t>(p) * VEC;
-            s[r][c].load(a.x + at);
-            if (a.residual != nullptr) res[r][c].load(a.residual + at);
+          if (row_live(r)) {
+            walk.load(s[r][c], a.x, r0 + r, c * NT + tid);
+            if (a.residual != nullptr) walk.load(res[r][c], a.residual, r0 + r, c * NT + tid);
           }
         }
 #pragma unroll
@@ -152,8 +252,9 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_kernel(const No
 #pragma unroll
             for (int i = 0; i < VEC; ++i) f[i] += v[i];
             s[r][c].set(f);
-            s[r][c].get(f);
           }
+          walk.mask(s[r][c], c * NT + tid);
+          s[r][c].get(f);
 #pragma unroll
           for (int i = 0; i < VEC; ++i) sq[r] = fmaf(f[i], f[i], sq[r]);
         }
@@ -170,21 +271,29 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_kernel(const No
 #pragma unroll
       for (int i = 0; i < VEC; ++i) y[i] = y[i] * rstd[r] * (a.weight != nullptr ? wf[i] : 1.f);
     };
-    auto live = [&](int r, int p) { return r < a.batch && r0 + r < a.rows && p < a.pieces; };
+    auto magnitude = [&](int r, int c) {  // the largest |y| of a piece; what lies outside the row is 0 unless rstd is not finite
+      float y[VEC], m = 0.f;
+      if (c * NT + tid >= walk.pieces) return m;
+      value(r, c, y);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        const int col = walk.col(c * NT + tid) + i;
+        if (!SHIFT || (col >= 0 && col < a.H)) m = MaxOp::join(m, fabsf(y[i]));
+      }
+      return m;
+    };
     if (MODE == kNorm) {
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-          const int p = c * NT + tid;
-          if (!live(r, p)) continue;
-          const int64_t at = (r0 + r) * a.H + static_cast<int64_t>(p) * VEC;
-          if (a.residual != nullptr) s[r][c].store(a.summed + at);
+          if (!row_live(r)) continue;
+          if (a.residual != nullptr) walk.store(s[r][c], a.summed + (r0 + r) * a.H, c * NT + tid);
           float y[VEC];
           value(r, c, y);
           Piece<T, VEC> out;
           out.set(y);
-          out.store(a.normed + at);
+          walk.store(out, a.normed + (r0 + r) * a.H, c * NT + tid);
         }
       continue;
     }
@@ -195,87 +304,99 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_kernel(const No
       for (int r = 0; r < R; ++r) {
         top[r] = 0.f;
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          float y[VEC];
-          if (!live(r, c * NT + tid)) continue;
-          value(r, c, y);
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) top[r] = MaxOp::join(top[r], fabsf(y[i]));
-        }
+        for (int c = 0; c < C; ++c) top[r] = MaxOp::join(top[r], magnitude(r, c));
       }
       group_join<MaxOp, WPG, R>(top, slots[g][2]);
     }
-    if (MODE == kFp8Block && VEC == 1) {
+    float most[R][C];
+    if (kTable) {
+      static_assert(!kTable || R == 1, "one table a group");
       uint32_t* m = block_max + g * a.groups;
       for (int i = tid; i < a.groups; i += NT) m[i] = 0;
       group_barrier<WPG>();
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         float y[VEC];
-        const int p = c * NT + tid;
-        if (!live(0, p)) continue;
+        const int col = walk.col(c * NT + tid);
+        if (c * NT + tid >= walk.pieces) continue;
         value(0, c, y);
-        atomicMax(m + (p >> a.group_shift), __float_as_uint(fabsf(y[0])));
+        // a piece has values of one block, or of two
+        const int block = (col > 0 ? col : 0) >> a.group_shift, next = (block + 1) << a.group_shift;
+        float here = 0.f, there = 0.f;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i)
+          if (col + i >= 0 && col + i < a.H) {
+            if (col + i < next) here = MaxOp::join(here, fabsf(y[i]));
+            else there = MaxOp::join(there, fabsf(y[i]));
+          }
+        atomicMax(m + block, __float_as_uint(here));
+        if (VEC > 1 && next < a.H && col + VEC > next) atomicMax(m + block + 1, __float_as_uint(there));
       }
       group_barrier<WPG>();
-    }
-    float most[R][C];
-    if (MODE == kFp8Block && VEC > 1) {
+    } else if (MODE == kFp8Block) {
       // a block is 4 to 32 neighbouring lanes
 #pragma unroll
       for (int r = 0; r < R; ++r)
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-          float y[VEC];
-          value(r, c, y);
-          most[r][c] = 0.f;
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) most[r][c] = MaxOp::join(most[r][c], fabsf(y[i]));
-        }
+        for (int c = 0; c < C; ++c) most[r][c] = magnitude(r, c);
       for (int d = (1 << a.group_shift) / (2 * VEC); d > 0; d >>= 1)
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
           for (int c = 0; c < C; ++c) most[r][c] = MaxOp::join(most[r][c], __shfl_xor_sync(kFull, most[r][c], d));
     }
+    auto scale_of = [&](float m) {
+      m *= 1.f / kE4m3Max;
+      return m < kMinScale ? kMinScale : m;  // a NaN stays
+    };
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int p = c * NT + tid;
-        const bool ok = live(r, p);
-        float y[VEC], m;
-        value(r, c, y);
-        const int col = p * VEC;
-        if (MODE == kFp8Row) m = top[r];
-        else if (VEC == 1) m = ok ? __uint_as_float(block_max[g * a.groups + (p >> a.group_shift)]) : 0.f;
-        else m = most[r][c];
-        if (!ok) continue;
-        m *= 1.f / kE4m3Max;
-        const float scale = m < kMinScale ? kMinScale : m;  // a NaN stays
-        const float inv = __fdividef(1.f, scale);           // 2^-126 <= scale < 2^120, or infinite: 0
-        const int64_t at = (r0 + r) * a.H + col;
-        if (MODE == kFp8Row) {
-          if (p == 0) a.scales[r0 + r] = scale;
-        } else if ((col & ((1 << a.group_shift) - 1)) == 0) {
-          a.scales[(r0 + r) * a.groups + (col >> a.group_shift)] = scale;
-        }
-        if (a.residual != nullptr) s[r][c].store(a.summed + at);
-        if (VEC == 1) {
-          a.q[at] = __nv_cvt_float_to_fp8(y[0] * inv, __NV_SATFINITE, __NV_E4M3);
+        const int p = c * NT + tid, col = walk.col(p);
+        if (!row_live(r) || p >= walk.pieces) continue;
+        const int64_t row = r0 + r;
+        const int block = (col > 0 ? col : 0) >> a.group_shift, next = (block + 1) << a.group_shift;
+        float m0, m1 = 0.f;
+        if (MODE == kFp8Row) m0 = top[r];
+        else if (kTable) {
+          m0 = __uint_as_float(block_max[g * a.groups + block]);
+          if (VEC > 1 && next < a.H) m1 = __uint_as_float(block_max[g * a.groups + block + 1]);
         } else {
-          uint16_t b[VEC / 2 + 1];
+          m0 = most[r][c];
+        }
+        const float scale = scale_of(m0);
+        // __fdividef: 2^-126 <= scale < 2^120, or infinite, where it gives 0
+        const float inv = __fdividef(1.f, scale), inv1 = kTable && VEC > 1 ? __fdividef(1.f, scale_of(m1)) : inv;
+        if (MODE == kFp8Row) {
+          if (p == 0) a.scales[row] = scale;
+        } else if (!kTable && (col & ((1 << a.group_shift) - 1)) == 0) {
+          a.scales[row * a.groups + block] = scale;
+        }
+        if (a.residual != nullptr) walk.template store<false>(s[r][c], a.summed + row * a.H, p);
+        float y[VEC];
+        value(r, c, y);
 #pragma unroll
-          for (int i = 0; i < VEC; i += 2)
-            b[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(y[i] * inv, y[i + (VEC > 1)] * inv), __NV_SATFINITE, __NV_E4M3);
-          if (VEC == 8)
-            *reinterpret_cast<uint2*>(a.q + at) = make_uint2(b[0] | (b[1] << 16), b[VEC / 4] | (b[3 * VEC / 8] << 16));
-          else
-            *reinterpret_cast<uint32_t*>(a.q + at) = b[0] | (b[1] << 16);
+        for (int i = 0; i < VEC; ++i) y[i] *= !kTable || col + i < next ? inv : inv1;
+        __nv_fp8_storage_t* q = a.q + row * a.H;
+        if (VEC > 1 && walk.whole(p)) {
+          uint32_t b[VEC > 1 ? VEC / 2 : 1];
+#pragma unroll
+          for (int i = 0; i + 1 < VEC; i += 2)
+            b[i / 2] = __nv_cvt_float2_to_fp8x2(make_float2(y[i], y[i + 1]), __NV_SATFINITE, __NV_E4M3);
+          if constexpr (VEC == 8) *reinterpret_cast<uint2*>(q + col) = make_uint2(b[0] | (b[1] << 16), b[2] | (b[3] << 16));
+          else if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(q + col) = b[0] | (b[1] << 16);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i)
+            if (i >= walk.lo(p) && i < walk.hi(p)) q[col + i] = __nv_cvt_float_to_fp8(y[i], __NV_SATFINITE, __NV_E4M3);
         }
       }
-    if (MODE == kFp8Block && VEC == 1) group_barrier<WPG>();  // block_max is cleared for the next row
-    if (MODE == kFp8Row && WPG > 1) group_barrier<WPG>();     // slots[g][2] is written again
+    if (kTable) {
+      for (int i = tid; i < a.groups; i += NT) a.scales[r0 * a.groups + i] = scale_of(__uint_as_float(block_max[g * a.groups + i]));
+      group_barrier<WPG>();  // the table is cleared for the next row
+    }
+    if (MODE == kFp8Row && WPG > 1) group_barrier<WPG>();  // slots[g][2] is written again
   }
 }
 
@@ -289,28 +410,25 @@ template <typename T> struct NormBackwardArgs {
   T* dx;
   float* part;  // nullable; [groups of the grid][H]
   int64_t rows;
-  int H, pieces, batch;
+  int H, batch;
   float eps;
 };
 
-template <typename T, int VEC, int WPG, int C, int R>
-__global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_backward_kernel(const NormBackwardArgs<T> a) {
+template <typename T, int VEC, int WPG, int C, int R, bool SHIFT>
+__global__ void __launch_bounds__(Group<WPG>::kCta, Group<WPG>::kCta > 256 || C > 2 ? 1 : 2) add_rms_norm_backward_kernel(const NormBackwardArgs<T> a) {
   constexpr int NT = Group<WPG>::kThreads;
   const int g = threadIdx.x / NT, tid = threadIdx.x % NT;
   __shared__ float slots[Group<WPG>::kPerCta][2][2 * R * WPG];
+  const Walk<VEC, WPG, SHIFT> walk(a.rows, a.H, a.batch);
   Piece<T, VEC> w[C];
   float dw[C][VEC];
 #pragma unroll
   for (int c = 0; c < C; ++c) {
-    const int p = c * NT + tid;
-    w[c].zero();
-    if (a.weight != nullptr && p < a.pieces) w[c].load(a.weight + static_cast<int64_t>(p) * VEC);
+    walk.weights(w[c], a.weight, c * NT + tid);
 #pragma unroll
     for (int i = 0; i < VEC; ++i) dw[c][i] = 0.f;
   }
   int turn = 0;
-  const int64_t slot = static_cast<int64_t>(blockIdx.x) * Group<WPG>::kPerCta + g;
-  const int64_t step = static_cast<int64_t>(gridDim.x) * Group<WPG>::kPerCta * a.batch;
   struct Batch {
     Piece<T, VEC> s[R][C], dn[R][C], ds[R][C];
   };
@@ -323,18 +441,19 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_backward_kernel
         b.s[r][c].zero();
         b.dn[r][c].zero();
         b.ds[r][c].zero();
-        if (r < a.batch && r0 + r < a.rows && p < a.pieces) {
-          const int64_t at = (r0 + r) * a.H + static_cast<int64_t>(p) * VEC;
-          b.s[r][c].load(a.summed + at);
-          b.dn[r][c].load(a.dnormed + at);
-          if (a.dsummed != nullptr) b.ds[r][c].load(a.dsummed + at);
+        if (R == 1 || (r < a.batch && r0 + r < a.rows)) {
+          walk.load(b.s[r][c], a.summed, r0 + r, p);
+          walk.load(b.dn[r][c], a.dnormed, r0 + r, p);
+          if (a.dsummed != nullptr) walk.load(b.ds[r][c], a.dsummed, r0 + r, p);
         }
       }
   };
+  // the next batch is on the way while this one is worked on, where the registers of a CTA hold both
+  constexpr bool kAhead = WPG * C * VEC <= 256;
   Batch now, next;
-  if (slot * a.batch < a.rows) fetch(slot * a.batch, now);
-  for (int64_t r0 = slot * a.batch; r0 < a.rows; r0 += step, turn ^= 1) {
-    if (r0 + step < a.rows) fetch(r0 + step, next);  // on the way while this batch is worked on
+  if (walk.row < a.rows) fetch(walk.row, now);
+  for (int64_t r0 = walk.row; r0 < a.rows; r0 += walk.step, turn ^= 1) {
+    if (kAhead && r0 + walk.step < a.rows) fetch(r0 + walk.step, next);
     auto& s = now.s;
     auto& dn = now.dn;
     auto& ds = now.ds;
@@ -345,6 +464,8 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_backward_kernel
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         float f[VEC], d[VEC], wf[VEC];
+        walk.mask(s[r][c], c * NT + tid);
+        walk.mask(dn[r][c], c * NT + tid);
         s[r][c].get(f);
         dn[r][c].get(d);
         w[c].get(wf);
@@ -364,8 +485,6 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_backward_kernel
       const float k = rstd * rstd * (sum[2 * r + 1] * inv_h);
 #pragma unroll
       for (int c = 0; c < C; ++c) {
-        const int p = c * NT + tid;
-        if (p >= a.pieces) continue;
         float f[VEC], d[VEC], e[VEC], wf[VEC], o[VEC];
         s[r][c].get(f);
         dn[r][c].get(d);
@@ -379,37 +498,42 @@ __global__ void __launch_bounds__(Group<WPG>::kCta) add_rms_norm_backward_kernel
         }
         Piece<T, VEC> out;
         out.set(o);
-        out.store(a.dx + (r0 + r) * a.H + static_cast<int64_t>(p) * VEC);
+        walk.store(out, a.dx + (r0 + r) * a.H, c * NT + tid);
       }
     }
-    now = next;
+    if (kAhead) now = next;
+    else if (r0 + walk.step < a.rows) fetch(r0 + walk.step, now);
   }
   if (a.part != nullptr) {
+    float* part = a.part + (static_cast<int64_t>(blockIdx.x) * Group<WPG>::kPerCta + g) * a.H;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int p = c * NT + tid;
-      if (p < a.pieces) {
+      const int col = walk.col(c * NT + tid);
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) a.part[slot * a.H + static_cast<int64_t>(p) * VEC + i] = dw[c][i];
-      }
+      for (int i = 0; i < VEC; ++i)
+        if (col + i >= 0 && col + i < a.H) part[col + i] = dw[c][i];
     }
   }
 }
 
-// dweight[c] = T(sum over the groups of part[group][c]), in a fixed order
+// dweight[c] = T(sum over the groups of part[group][c]), in a fixed order: a warp takes every 32nd group
 template <typename T>
-__global__ void __launch_bounds__(256) rms_norm_dweight_kernel(const float* part, int groups, int H, T* dweight) {
-  __shared__ float sums[8][32];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), w = threadIdx.x >> 5;
+__global__ void __launch_bounds__(1024) rms_norm_dweight_kernel(const float* part, int groups, int H, T* dweight) {
+  __shared__ float sums[32][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
   float v = 0.f;
-  if (c < H)
-    for (int i = w; i < groups; i += 8) v += part[static_cast<int64_t>(i) * H + c];
-  sums[w][threadIdx.x & 31] = v;
-  __syncthreads();
-  if (w == 0 && c < H) {
-    for (int i = 1; i < 8; ++i) v += sums[i][threadIdx.x];
-    dweight[c] = from_f32<T>(v);
+  if (c < H) {
+#pragma unroll 8
+    for (int i = w; i < groups; i += 32) v += part[static_cast<int64_t>(i) * H + c];
   }
+  sums[w][lane] = v;
+  __syncthreads();
+  v = sums[lane][w];  // warp w adds up column w of the block
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(kFull, v, d);
+  const int out = blockIdx.x * 32 + w;
+  if (lane == 0 && out < H) dweight[out] = from_f32<T>(v);
 }
 
 constexpr int kMaxHidden = 16384;
@@ -421,7 +545,7 @@ struct Shape {
 };
 #define FMOE_VEC_SHAPES(X) X(0, 1, 1, 4, 2) X(1, 1, 2, 1, 1) X(2, 2, 2, 1, 1) X(3, 4, 2, 1, 1) X(4, 8, 2, 1, 1) X(5, 8, 4, 1, 1) \
   X(6, 16, 4, 1, 1) X(7, 32, 4, 1, 1)
-#define FMOE_ONE_SHAPES(X) X(0, 1, 8, 1, 1) X(1, 8, 8, 1, 1) X(2, 32, 16, 1, 1)
+#define FMOE_ONE_SHAPES(X) X(0, 1, 8, 1, 1) X(1, 8, 8, 1, 1) X(2, 16, 16, 1, 1) X(3, 32, 16, 1, 1)
 #define FMOE_SHAPE(I_, W_, C_, RF_, RB_) {W_, C_},
 constexpr Shape kVecShapes[] = {FMOE_VEC_SHAPES(FMOE_SHAPE)};
 constexpr Shape kOneShapes[] = {FMOE_ONE_SHAPES(FMOE_SHAPE)};
@@ -437,11 +561,11 @@ int shape_of(bool vec, int pieces) {
 }
 
 // Groups that the grid of a backward has: all that its registers let run at once, and no more, since each group leaves a row of
-// partial sums.
+// partial sums.  A multiple of eight, so that SHIFT keeps its remainders.
 int64_t backward_groups(Shape sh, int64_t rows) {
   const int cta = sh.wpg < 8 ? 256 : 32 * sh.wpg, per_cta = cta / (32 * sh.wpg);
-  const int64_t cap = static_cast<int64_t>(device_sm_count()) * (sh.wpg * sh.c <= 16 ? 2 : 1) * per_cta;
-  return rows < cap ? (rows + per_cta - 1) / per_cta * per_cta : cap;
+  const int64_t cap = static_cast<int64_t>(device_sm_count()) * (sh.wpg * sh.c <= 16 ? 2 : 1) * per_cta / 8 * 8;
+  return rows < cap ? (rows + 7) / 8 * 8 : cap;
 }
 
 // rows a group takes at a time: as many as fit its registers once every SM has a group, fewer before
@@ -450,48 +574,64 @@ int batch_rows(int64_t rows, int most, int per_cta) {
   return static_cast<int>(each < 1 ? 1 : each < most ? each : most);
 }
 
-template <typename T, int VEC, int WPG, int C, int R>
+template <typename T, int VEC, int WPG, int C, int R, bool SHIFT>
 int launch_forward(const NormArgs<T>& in, int mode, cudaStream_t stream) {
   NormArgs<T> a = in;
   constexpr int per_cta = Group<WPG>::kPerCta;
   a.batch = batch_rows(a.rows, R, per_cta);
-  const int64_t want = (a.rows + static_cast<int64_t>(a.batch) * per_cta - 1) / (static_cast<int64_t>(a.batch) * per_cta);
+  int64_t grid = (a.rows + static_cast<int64_t>(a.batch) * per_cta - 1) / (static_cast<int64_t>(a.batch) * per_cta);
   const int64_t cap = static_cast<int64_t>(device_sm_count()) * 8;
-  const unsigned grid = static_cast<unsigned>(want < cap ? want : cap);
-  const int smem = mode == kFp8Block && VEC == 1 ? per_cta * a.groups * 4 : 0;
-  if (mode == kNorm) add_rms_norm_kernel<T, VEC, WPG, C, R, kNorm><<<grid, Group<WPG>::kCta, 0, stream>>>(a);
-  else if (mode == kFp8Row) add_rms_norm_kernel<T, VEC, WPG, C, R, kFp8Row><<<grid, Group<WPG>::kCta, 0, stream>>>(a);
-  else add_rms_norm_kernel<T, VEC, WPG, C, R, kFp8Block><<<grid, Group<WPG>::kCta, smem, stream>>>(a);
+  if (grid > cap) grid = cap;
+  if (SHIFT) grid = (grid + 7) / 8 * 8;
+  const unsigned ctas = static_cast<unsigned>(grid);
+  const int smem = mode == kFp8Block && (VEC == 1 || SHIFT) ? per_cta * a.groups * 4 : 0;
+  if (mode == kNorm) add_rms_norm_kernel<T, VEC, WPG, C, R, SHIFT, kNorm><<<ctas, Group<WPG>::kCta, 0, stream>>>(a);
+  else if (mode == kFp8Row) add_rms_norm_kernel<T, VEC, WPG, C, R, SHIFT, kFp8Row><<<ctas, Group<WPG>::kCta, 0, stream>>>(a);
+  else add_rms_norm_kernel<T, VEC, WPG, C, R, SHIFT, kFp8Block><<<ctas, Group<WPG>::kCta, smem, stream>>>(a);
   FMOE_LAUNCH_CHECK();
   return FMOE_OK;
 }
 
-template <typename T, int VEC, int WPG, int C, int R>
+template <typename T, int VEC, int WPG, int C, int R, bool SHIFT>
 int launch_backward(const NormBackwardArgs<T>& in, T* dweight, cudaStream_t stream) {
   NormBackwardArgs<T> a = in;
   constexpr int per_cta = Group<WPG>::kPerCta;
   a.batch = batch_rows(a.rows, R, per_cta);
   const int64_t groups = backward_groups({WPG, C}, a.rows);
-  add_rms_norm_backward_kernel<T, VEC, WPG, C, R><<<static_cast<unsigned>(groups / per_cta), Group<WPG>::kCta, 0, stream>>>(a);
+  add_rms_norm_backward_kernel<T, VEC, WPG, C, R, SHIFT><<<static_cast<unsigned>(groups / per_cta), Group<WPG>::kCta, 0, stream>>>(a);
   FMOE_LAUNCH_CHECK();
   if (dweight != nullptr) {
-    rms_norm_dweight_kernel<T><<<(a.H + 31) / 32, 256, 0, stream>>>(a.part, static_cast<int>(groups), a.H, dweight);
+    rms_norm_dweight_kernel<T><<<(a.H + 31) / 32, 1024, 0, stream>>>(a.part, static_cast<int>(groups), a.H, dweight);
     FMOE_LAUNCH_CHECK();
   }
   return FMOE_OK;
 }
 
+// kWhole: rows of aligned pieces; kShifted: rows of any length in memory that starts at a piece; kSingle: one value at a time
+enum Form { kWhole, kShifted, kSingle };
+constexpr int kMostPieces = 4096;  // of the widest shape
+// pieces of a row, at most
+int pieces_of(Form form, int vec, int H) { return form == kSingle ? H : form == kWhole ? H / vec : (H + 2 * vec - 2) / vec; }
+Form form_of(int vec, int H, std::initializer_list<const void*> pointers) {
+  for (const void* p : pointers)
+    if (!aligned16(p)) return kSingle;
+  return H % vec == 0 ? kWhole : pieces_of(kShifted, vec, H) <= kMostPieces ? kShifted : kSingle;
+}
+
 template <typename T>
 int forward_typed(const void* x, const void* residual, const void* weight, void* summed, void* normed, void* q, float* scales,
                   int64_t rows, int H, int group, float eps, int mode, cudaStream_t stream) {
-  const bool vec = H % Vec16<T>::N == 0 && aligned16(x) && aligned16(residual) && aligned16(weight) && aligned16(summed) &&
-                   aligned16(normed) && aligned16(q);
-  NormArgs<T> a = {static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight),
-                   static_cast<T*>(summed), static_cast<T*>(normed), static_cast<__nv_fp8_storage_t*>(q), scales, rows, H,
-                   vec ? H / Vec16<T>::N : H, 1, group == 32 ? 5 : group == 64 ? 6 : 7, mode == kFp8Block ? (H + group - 1) / group : 1, eps};
-  const int shape = shape_of(vec, a.pieces);
-#define FMOE_VEC(I_, W_, C_, RF_, RB_) if (vec && shape == I_) return launch_forward<T, Vec16<T>::N, W_, C_, RF_>(a, mode, stream);
-#define FMOE_ONE(I_, W_, C_, RF_, RB_) if (!vec && shape == I_) return launch_forward<T, 1, W_, C_, RF_>(a, mode, stream);
+  constexpr int V = Vec16<T>::N;
+  Form form = form_of(V, H, {x, residual, summed, normed, q});
+  if (form == kWhole && !aligned16(weight)) form = kShifted;  // which reads weights one by one
+  const NormArgs<T> a = {static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight),
+                         static_cast<T*>(summed), static_cast<T*>(normed), static_cast<__nv_fp8_storage_t*>(q), scales, rows, H, 1,
+                         group == 32 ? 5 : group == 64 ? 6 : 7, mode == kFp8Block ? (H + group - 1) / group : 1, eps};
+  const int shape = shape_of(form != kSingle, pieces_of(form, V, H));
+#define FMOE_VEC(I_, W_, C_, RF_, RB_)                                                                    \
+  if (form == kWhole && shape == I_) return launch_forward<T, V, W_, C_, RF_, false>(a, mode, stream);    \
+  if (form == kShifted && shape == I_) return launch_forward<T, V, W_, C_, 1, true>(a, mode, stream);
+#define FMOE_ONE(I_, W_, C_, RF_, RB_) if (form == kSingle && shape == I_) return launch_forward<T, 1, W_, C_, RF_, false>(a, mode, stream);
   FMOE_VEC_SHAPES(FMOE_VEC)
   FMOE_ONE_SHAPES(FMOE_ONE)
 #undef FMOE_VEC
@@ -499,20 +639,20 @@ int forward_typed(const void* x, const void* residual, const void* weight, void*
   return FMOE_ERR_UNSUPPORTED;
 }
 
-bool backward_vec(int dtype, int H, const void* a, const void* b, const void* c, const void* d, const void* e) {
-  return H % (16 / dtype_size(dtype)) == 0 && aligned16(a) && aligned16(b) && aligned16(c) && aligned16(d) && aligned16(e);
-}
-
 template <typename T>
 int backward_typed(const void* dnormed, const void* dsummed, const void* summed, const void* weight, void* dx, void* dweight,
-                   float* part, bool vec, int64_t rows, int H, float eps, cudaStream_t stream) {
-  NormBackwardArgs<T> a = {static_cast<const T*>(dnormed), static_cast<const T*>(dsummed), static_cast<const T*>(summed),
-                           static_cast<const T*>(weight), static_cast<T*>(dx), dweight != nullptr ? part : nullptr, rows, H,
-                           vec ? H / Vec16<T>::N : H, 1, eps};
+                   float* part, int64_t rows, int H, float eps, cudaStream_t stream) {
+  constexpr int V = Vec16<T>::N;
+  Form form = form_of(V, H, {dnormed, dsummed, summed, dx});
+  if (form == kWhole && !aligned16(weight)) form = kShifted;
+  const NormBackwardArgs<T> a = {static_cast<const T*>(dnormed), static_cast<const T*>(dsummed), static_cast<const T*>(summed),
+                                 static_cast<const T*>(weight), static_cast<T*>(dx), dweight != nullptr ? part : nullptr, rows, H, 1, eps};
   T* dw = static_cast<T*>(dweight);
-  const int shape = shape_of(vec, a.pieces);
-#define FMOE_VEC(I_, W_, C_, RF_, RB_) if (vec && shape == I_) return launch_backward<T, Vec16<T>::N, W_, C_, RB_>(a, dw, stream);
-#define FMOE_ONE(I_, W_, C_, RF_, RB_) if (!vec && shape == I_) return launch_backward<T, 1, W_, C_, RB_>(a, dw, stream);
+  const int shape = shape_of(form != kSingle, pieces_of(form, V, H));
+#define FMOE_VEC(I_, W_, C_, RF_, RB_)                                                                    \
+  if (form == kWhole && shape == I_) return launch_backward<T, V, W_, C_, RB_, false>(a, dw, stream);     \
+  if (form == kShifted && shape == I_) return launch_backward<T, V, W_, C_, 1, true>(a, dw, stream);
+#define FMOE_ONE(I_, W_, C_, RF_, RB_) if (form == kSingle && shape == I_) return launch_backward<T, 1, W_, C_, RB_, false>(a, dw, stream);
   FMOE_VEC_SHAPES(FMOE_VEC)
   FMOE_ONE_SHAPES(FMOE_ONE)
 #undef FMOE_VEC
@@ -540,14 +680,16 @@ int launch_add_rms_norm(const void* x, const void* residual, const void* weight,
   }
 }
 
-// the larger of what the two forms of a call (16-byte pieces, single values) use
+// the largest of what the forms of a call use
 size_t add_rms_norm_backward_workspace_bytes(int64_t rows, int H, int dtype) {
   if (rows <= 0 || H <= 0 || H > kMaxHidden) return 0;
   const int n = 16 / dtype_size(dtype);
-  int64_t groups = backward_groups(kOneShapes[shape_of(false, H)], rows);
-  if (H % n == 0) {
-    const int64_t v = backward_groups(kVecShapes[shape_of(true, H / n)], rows);
-    groups = v > groups ? v : groups;
+  int64_t groups = 0;
+  for (const Form form : {kWhole, kShifted, kSingle}) {
+    if (form != kSingle && pieces_of(form, n, H) > kMostPieces) continue;
+    const Shape sh = form == kSingle ? kOneShapes[shape_of(false, H)] : kVecShapes[shape_of(true, pieces_of(form, n, H))];
+    const int64_t g = backward_groups(sh, rows);
+    groups = g > groups ? g : groups;
   }
   return static_cast<size_t>(groups) * H * sizeof(float);
 }
@@ -563,12 +705,11 @@ int launch_add_rms_norm_backward(const void* dnormed, const void* dsummed, const
   }
   if (dnormed == nullptr || summed == nullptr || dx == nullptr) return FMOE_ERR_BAD_ARG;
   if (dweight != nullptr && (ws == nullptr || ws_bytes < add_rms_norm_backward_workspace_bytes(rows, H, dtype))) return FMOE_ERR_WORKSPACE;
-  const bool vec = backward_vec(dtype, H, dnormed, dsummed, summed, weight, dx);
   float* part = static_cast<float*>(ws);
   switch (dtype) {
-    case FMOE_DTYPE_F32: return backward_typed<float>(dnormed, dsummed, summed, weight, dx, dweight, part, vec, rows, H, eps, stream);
-    case FMOE_DTYPE_BF16: return backward_typed<__nv_bfloat16>(dnormed, dsummed, summed, weight, dx, dweight, part, vec, rows, H, eps, stream);
-    case FMOE_DTYPE_F16: return backward_typed<__half>(dnormed, dsummed, summed, weight, dx, dweight, part, vec, rows, H, eps, stream);
+    case FMOE_DTYPE_F32: return backward_typed<float>(dnormed, dsummed, summed, weight, dx, dweight, part, rows, H, eps, stream);
+    case FMOE_DTYPE_BF16: return backward_typed<__nv_bfloat16>(dnormed, dsummed, summed, weight, dx, dweight, part, rows, H, eps, stream);
+    case FMOE_DTYPE_F16: return backward_typed<__half>(dnormed, dsummed, summed, weight, dx, dweight, part, rows, H, eps, stream);
     default: return FMOE_ERR_BAD_ARG;
   }
 }

@@ -17,7 +17,7 @@ namespace {
 constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr int kTensors = 96;
 constexpr int kThreads = 256;
-constexpr int kChunkBytes = 16384;  // four 16-byte loads a thread
+constexpr int kChunkBytes = 32768;  // eight 16-byte loads a thread
 constexpr int kLoads = kChunkBytes / 16 / kThreads;
 
 struct TensorList {
@@ -28,10 +28,6 @@ struct TensorList {
   int count;
 };
 
-struct Chunk {
-  int tensor;
-  int64_t at;  // index of the chunk in its tensor
-};
 // the tensor that chunk c belongs to
 __device__ __forceinline__ int find_tensor(const TensorList& l, int64_t c) {
   int lo = 0, hi = l.count - 1;
@@ -43,37 +39,52 @@ __device__ __forceinline__ int find_tensor(const TensorList& l, int64_t c) {
   return lo;
 }
 
-template <typename T> __device__ __forceinline__ float chunk_squares(const T* p, int64_t numel, int64_t chunk) {
+// A CTA's walk over its chunks, up or down, with the next chunk's pieces on the way while the present one is worked on.  Pieces are
+// raw 16 bytes whatever the type; a tensor that does not start at one is read value by value.
+struct Walk {
+  const TensorList& l;
+  int tensor;
+  uint4 q[kLoads];
+  char* at;   // the chunk
+  int bytes;  // of it
+  uint8_t dtype;
+  bool pieces;
+
+  __device__ __forceinline__ Walk(const TensorList& list, int64_t c) : l(list), tensor(find_tensor(list, c)) {}
+  __device__ __forceinline__ void fetch(int64_t c) {
+    while (c >= l.first[tensor + 1]) ++tensor;
+    while (c < l.first[tensor]) --tensor;
+    dtype = l.dtype[tensor];
+    const int64_t offset = (c - l.first[tensor]) * kChunkBytes;
+    const int64_t left = l.numel[tensor] * (dtype == FMOE_DTYPE_F32 ? 4 : 2) - offset;
+    at = static_cast<char*>(l.ptr[tensor]) + offset;
+    bytes = static_cast<int>(left < kChunkBytes ? left : kChunkBytes);
+    pieces = (reinterpret_cast<uintptr_t>(at) & 15u) == 0;
+#pragma unroll
+    for (int i = 0; i < kLoads; ++i) {
+      const int b = (i * kThreads + threadIdx.x) * 16;
+      q[i] = make_uint4(0, 0, 0, 0);
+      if (pieces && b + 16 <= bytes) q[i] = ld16(at + b);
+    }
+  }
+  // values that are not in a whole piece: from(index), then every kThreads
+  __device__ __forceinline__ int rest(int size) const { return (pieces ? bytes / 16 * 16 / size : 0) + threadIdx.x; }
+};
+
+template <typename T> __device__ __forceinline__ float chunk_squares(const Walk& w) {
   constexpr int VEC = Vec16<T>::N;
-  constexpr int kElems = kChunkBytes / sizeof(T);
-  const int64_t e0 = chunk * kElems;
-  const int n = static_cast<int>(numel - e0 < kElems ? numel - e0 : kElems);
-  p += e0;
   float acc[4] = {0.f, 0.f, 0.f, 0.f};
-  if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
-    uint4 q[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int e = (i * kThreads + threadIdx.x) * VEC;
-      q[i] = e + VEC <= n ? ld16(p + e) : make_uint4(0, 0, 0, 0);
-    }
+  for (int i = 0; i < kLoads; ++i) {
+    float f[VEC];
+    unpack16<T>(w.q[i], f);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      float f[VEC];
-      unpack16<T>(q[i], f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) acc[j & 3] = fmaf(f[j], f[j], acc[j & 3]);
-    }
-    const int e = n / VEC * VEC + threadIdx.x;
-    if (e < n) {
-      const float f = to_f32<T>(p[e]);
-      acc[0] = fmaf(f, f, acc[0]);
-    }
-  } else {
-    for (int e = threadIdx.x; e < n; e += kThreads) {
-      const float f = to_f32<T>(p[e]);
-      acc[0] = fmaf(f, f, acc[0]);
-    }
+    for (int j = 0; j < VEC; ++j) acc[j & 3] = fmaf(f[j], f[j], acc[j & 3]);
+  }
+  const T* p = reinterpret_cast<const T*>(w.at);
+  for (int e = w.rest(sizeof(T)); e < static_cast<int>(w.bytes / sizeof(T)); e += kThreads) {
+    const float f = to_f32<T>(p[e]);
+    acc[0] = fmaf(f, f, acc[0]);
   }
   return (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }
@@ -93,16 +104,19 @@ __device__ __forceinline__ double cta_sum(double v) {
 __global__ void __launch_bounds__(kThreads) grad_squares_kernel(const __grid_constant__ TensorList l, double* part) {
   const int64_t chunks = l.first[l.count];
   const int64_t c0 = chunks * blockIdx.x / gridDim.x, c1 = chunks * (blockIdx.x + 1) / gridDim.x;
-  int t = find_tensor(l, c0);
   double sum = 0.0;  // float32 inside a chunk, 64 bits over the chunks
-  for (int64_t c = c0; c < c1; ++c) {
-    while (c >= l.first[t + 1]) ++t;
-    const int64_t at = c - l.first[t];
-    float v;
-    if (l.dtype[t] == FMOE_DTYPE_F32) v = chunk_squares(static_cast<const float*>(l.ptr[t]), l.numel[t], at);
-    else if (l.dtype[t] == FMOE_DTYPE_BF16) v = chunk_squares(static_cast<const __nv_bfloat16*>(l.ptr[t]), l.numel[t], at);
-    else v = chunk_squares(static_cast<const __half*>(l.ptr[t]), l.numel[t], at);
-    sum += v;
+  if (c0 < c1) {
+    Walk next(l, c0);
+    next.fetch(c0);
+    for (int64_t c = c0; c < c1; ++c) {
+      const Walk now = next;
+      if (c + 1 < c1) next.fetch(c + 1);
+      float v;
+      if (now.dtype == FMOE_DTYPE_F32) v = chunk_squares<float>(now);
+      else if (now.dtype == FMOE_DTYPE_BF16) v = chunk_squares<__nv_bfloat16>(now);
+      else v = chunk_squares<__half>(now);
+      sum += v;
+    }
   }
   sum = cta_sum(sum);
   if (threadIdx.x == 0) part[blockIdx.x] = sum;
@@ -130,34 +144,19 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const NormArgs a) {
   if (threadIdx.x == 0) *a.norm = n;
 }
 
-template <typename T> __device__ __forceinline__ void chunk_scale(T* p, int64_t numel, int64_t chunk, float factor) {
+template <typename T> __device__ __forceinline__ void chunk_scale(const Walk& w, float factor) {
   constexpr int VEC = Vec16<T>::N;
-  constexpr int kElems = kChunkBytes / sizeof(T);
-  const int64_t e0 = chunk * kElems;
-  const int n = static_cast<int>(numel - e0 < kElems ? numel - e0 : kElems);
-  p += e0;
-  if ((reinterpret_cast<uintptr_t>(p) & 15u) == 0) {
-    uint4 q[kLoads];
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int e = (i * kThreads + threadIdx.x) * VEC;
-      if (e + VEC <= n) q[i] = ld16(p + e);
-    }
+  for (int i = 0; i < kLoads; ++i) {
+    const int b = (i * kThreads + threadIdx.x) * 16;
+    float f[VEC];
+    unpack16<T>(w.q[i], f);
 #pragma unroll
-    for (int i = 0; i < kLoads; ++i) {
-      const int e = (i * kThreads + threadIdx.x) * VEC;
-      if (e + VEC > n) continue;
-      float f[VEC];
-      unpack16<T>(q[i], f);
-#pragma unroll
-      for (int j = 0; j < VEC; ++j) f[j] *= factor;
-      *reinterpret_cast<uint4*>(p + e) = pack16<T>(f);
-    }
-    const int e = n / VEC * VEC + threadIdx.x;
-    if (e < n) p[e] = from_f32<T>(to_f32<T>(p[e]) * factor);
-  } else {
-    for (int e = threadIdx.x; e < n; e += kThreads) p[e] = from_f32<T>(to_f32<T>(p[e]) * factor);
+    for (int j = 0; j < VEC; ++j) f[j] *= factor;
+    if (w.pieces && b + 16 <= w.bytes) *reinterpret_cast<uint4*>(w.at + b) = pack16<T>(f);
   }
+  T* p = reinterpret_cast<T*>(w.at);
+  for (int e = w.rest(sizeof(T)); e < static_cast<int>(w.bytes / sizeof(T)); e += kThreads) p[e] = from_f32<T>(to_f32<T>(p[e]) * factor);
 }
 
 // Chunks in the opposite order of the sums: what those read last is in the L2 cache still.
@@ -172,17 +171,18 @@ __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_const
   const int64_t chunks = l.first[l.count];
   const int64_t c0 = chunks * blockIdx.x / gridDim.x, c1 = chunks * (blockIdx.x + 1) / gridDim.x;
   if (c0 == c1) return;
-  int t = find_tensor(l, c1 - 1);
+  Walk next(l, c1 - 1);
+  next.fetch(c1 - 1);
   for (int64_t c = c1 - 1; c >= c0; --c) {
-    while (c < l.first[t]) --t;
-    const int64_t at = c - l.first[t];
-    if (l.dtype[t] == FMOE_DTYPE_F32) chunk_scale(static_cast<float*>(l.ptr[t]), l.numel[t], at, factor);
-    else if (l.dtype[t] == FMOE_DTYPE_BF16) chunk_scale(static_cast<__nv_bfloat16*>(l.ptr[t]), l.numel[t], at, factor);
-    else chunk_scale(static_cast<__half*>(l.ptr[t]), l.numel[t], at, factor);
+    const Walk now = next;
+    if (c > c0) next.fetch(c - 1);
+    if (now.dtype == FMOE_DTYPE_F32) chunk_scale<float>(now, factor);
+    else if (now.dtype == FMOE_DTYPE_BF16) chunk_scale<__nv_bfloat16>(now, factor);
+    else chunk_scale<__half>(now, factor);
   }
 }
 
-int grid_cap() { return device_sm_count() * 4; }
+int grid_cap() { return device_sm_count() * 2; }
 int launches(int count) { return (count + kTensors - 1) / kTensors; }
 
 // no two tensors may share memory: one would be scaled twice
