@@ -10,7 +10,7 @@ from __future__ import annotations
 import ctypes
 import math
 import warnings
-from typing import Dict, Optional, Tuple
+from typing import Dict, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -182,6 +182,21 @@ class FlashMoE(nn.Module):
         if return_routing:
             self.last_indices, self.last_gates = indices, gates.detach()
         return (shared + experts).view(bsz, seq_len, -1), router_logits
+
+    def balance_loss(self, router_logits: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """`flash_moe_b200.balance_loss` of the logits that a forward with ``return_routing=True`` returned, with the counts of
+        the ids that it selected (``last_indices``; call it before the next such forward)."""
+        from ..ops.balance import balance_loss, expert_counts
+
+        if self.last_indices is None or router_logits.dim() != 3 or self.last_indices.shape[0] != router_logits.shape[1]:
+            raise _lib.FmoeError("balance_loss needs the logits of the last forward with return_routing=True")
+        return balance_loss(router_logits, expert_counts(self.last_indices, self.num_experts, token_mask), token_mask)
+
+    def clip_grad_norm_(self, max_norm: float, grad_scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
+        """`flash_moe_b200.clip_grad_norm_` for the parameters of the layer."""
+        from ..ops.grad_clip import clip_grad_norm_
+
+        return clip_grad_norm_(self.parameters(), max_norm, grad_scale)
 
     def forward(
         self,

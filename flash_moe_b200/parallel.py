@@ -84,7 +84,12 @@ def choose_hot_experts(indices: torch.Tensor, num_experts: int, count: int, grou
     id.  Under a skewed popularity a few hundred experts hold most pairs; copying their rows to every GPU keeps
     those pairs off the wire.  Collective: every rank of `group` calls it."""
     valid = (indices >= 0) & (indices < num_experts)
-    hist = torch.bincount(indices[valid].reshape(-1), minlength=num_experts).to(torch.int64)
+    if indices.is_cuda:  # without the host's wait for the size of indices[valid]
+        from .ops.balance import expert_counts
+
+        hist = expert_counts(torch.where(valid, indices, -1).reshape(-1, 1), num_experts)
+    else:
+        hist = torch.bincount(indices[valid].reshape(-1), minlength=num_experts).to(torch.int64)
     if dist.is_initialized() and dist.get_world_size(group) > 1:
         dist.all_reduce(hist, group=group)
     count = min(count, num_experts)

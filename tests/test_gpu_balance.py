@@ -138,7 +138,7 @@ def check(T, nk, k, dtype, masked=0.0, seed=0, upstream=1.0, counts=None, logits
     assert loss.shape == () and loss.dtype == torch.float32
     (got,) = torch.autograd.grad(loss, logits, torch.tensor(upstream, device="cuda"))
     want_loss, loss_slack, want, slack = reference(logits, counts, mask, upstream)
-    assert abs(float(loss) - want_loss) <= loss_slack
+    assert abs(loss.item() - want_loss) <= loss_slack
     fi = torch.finfo(logits.dtype)
     bound = slack + (want.abs() + slack) * fi.eps / 2 + fi.tiny * fi.eps
     off = (got.double() - want).abs()
