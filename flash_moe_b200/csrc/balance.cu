@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const int6
 
 // Many selections of not too many experts: every CTA counts all its selections in shared memory, in 16 bits an expert, and the
 // eight CTAs of a cluster add theirs up before they go to global memory, each a part of the experts and in ascending order.
-// At 4.2 million selections of 65536 experts the tables above are mostly taken by others: 47 us, by this kernel XX.
+// At 4.2 million selections of 65536 experts the tables above are mostly taken by others: 30 us, by this kernel 21.
 constexpr int kHistCtas = 8;
 constexpr int kHistThreads = 1024;
 constexpr int kHistExperts = 102400;      // 200 KB
@@ -185,12 +185,25 @@ struct Prepared {
 };
 constexpr size_t kHeadBytes = 256;
 
-// exp(t) for t <= 0 by the exponential of base 2: within a few 2^-23 of it, values below 2^-126 become 0
-__device__ __forceinline__ float exp_below(float t) {
-  float v;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(t * 1.44269504f));
-  return v;
-}
+// exp(x - top) / 2^d, with one small d for all values of a row whose largest is top: by the exponential of base 2, at
+// x log2 e - c, where c is top log2 e rounded and d what it was rounded by, which the row's sum has as well.  One multiply-add and
+// one exponential; values below 2^-126 become 0.  From 2^30 on d would overflow: neighbours of type float are 64 or more apart
+// there, so x = top is all that counts, and a power of two in the place of log2 e, for which c is exact, gives 1 for it and 0 for
+// the others, 256 below it.
+struct RowExp {
+  float a, c;
+  __device__ __forceinline__ explicit RowExp(float top) {
+    const int e = static_cast<int>(__float_as_uint(top) >> 23 & 255u) - 127;
+    a = e < 30 ? 1.44269504f : __uint_as_float(static_cast<uint32_t>(32 - e + 127) << 23);
+    c = __fmul_rn(a, top);
+  }
+  __device__ __forceinline__ RowExp() : a(0.f), c(0.f) {}
+  __device__ __forceinline__ float operator()(float x) const {
+    float v;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(v) : "f"(fmaf(x, a, -c)));
+    return v;
+  }
+};
 
 template <typename T> __device__ __forceinline__ uint32_t minus_infinity() { return 0xFF800000u; }
 template <> __device__ __forceinline__ uint32_t minus_infinity<__nv_bfloat16>() { return 0xFF80FF80u; }
@@ -219,7 +232,16 @@ template <typename T, bool VEC> __device__ __forceinline__ uint4 load_piece(cons
   const uint32_t none = minus_infinity<T>();
   uint4 q = make_uint4(none, none, none, none);
   if constexpr (VEC) {
-    if (read && c < nk) q = ld16(row + c);
+    // one predicated load into the registers that hold the fill: with a branch, the compiler may copy the value where the ways
+    // meet, and a copy waits for it
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        "setp.ne.s32 p, %5, 0;\n\t"
+        "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t"
+        "}\n"
+        : "+r"(q.x), "+r"(q.y), "+r"(q.z), "+r"(q.w)
+        : "l"(__cvta_generic_to_global(row + c)), "r"(static_cast<int>(read && c < nk)));
   } else {
     T v[N];
 #pragma unroll
@@ -227,6 +249,27 @@ template <typename T, bool VEC> __device__ __forceinline__ uint4 load_piece(cons
     memcpy(&q, v, 16);
   }
   return q;
+}
+// likewise: what is not read stays as it was
+__device__ __forceinline__ void load_if(bool read, const float* at, float& x, float& y) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.s32 p, %3, 0;\n\t"
+      "@p ld.global.v2.f32 {%0, %1}, [%2];\n\t"
+      "}\n"
+      : "+f"(x), "+f"(y)
+      : "l"(__cvta_generic_to_global(at)), "r"(static_cast<int>(read)));
+}
+__device__ __forceinline__ void load_if(bool read, const float* at, float& x) {
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p;\n\t"
+      "setp.ne.s32 p, %2, 0;\n\t"
+      "@p ld.global.f32 %0, [%1];\n\t"
+      "}\n"
+      : "+f"(x)
+      : "l"(__cvta_generic_to_global(at)), "r"(static_cast<int>(read)));
 }
 template <typename T, bool VEC> __device__ __forceinline__ void store_piece(T* row, int c, int nk, const uint4& q) {
   constexpr int N = Vec16<T>::N;
@@ -320,11 +363,12 @@ __global__ void __launch_bounds__(256, 4) balance_stats_kernel(const T* logits, 
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       float part[4] = {0.f, 0.f, 0.f, 0.f};
+      const RowExp exp_of(top[h]);
       auto join = [&](const uint4& v) {
         float f[N];
         unpack16<T>(v, f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) part[i & 3] += exp_below(f[i] - top[h]);
+        for (int i = 0; i < N; ++i) part[i & 3] += exp_of(f[i]);
       };
 #pragma unroll
       for (int u = 0; u < HELD; ++u) join(q[h][u]);
@@ -344,7 +388,8 @@ __global__ void __launch_bounds__(256, 4) balance_stats_kernel(const T* logits, 
 
 // Matrix h [row n][column k]: what multiplies p_(1-h)[k] in G_h[n], so h = 0 is C and h = 1 its transpose.  Stored in blocks of 64
 // columns, [k / 64][n][64], each row 128 bytes with its 16-byte pieces swizzled as the tensor core reads them: a block of rows is
-// copied to shared memory as it is.
+// copied to shared memory as it is.  Each 32 rows, the columns of the product, are in the order in which four threads read eight
+// neighbouring columns each out of tensor memory (ptx::tmem_ld_32x256): column 8 q + 2 j + b is at 8 j + 2 q + b.
 __global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* counts, int nk, int padded, const Part* part, Prepared* head,
                                                               uint4* pieces) {
   pdl_launch_dependents();
@@ -405,7 +450,8 @@ __global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* cou
     hi[i] = v;
     lo[i] = rest;
   }
-  const int64_t slot = (static_cast<int64_t>(col / 64) * padded + row) * 8 + (((col % 64) / 8) ^ (row & 7));
+  const int at_row = (row & ~31) | (((row >> 1) & 3) << 3) | (((row >> 3) & 3) << 1) | (row & 1);
+  const int64_t slot = (static_cast<int64_t>(col / 64) * padded + at_row) * 8 + (((col % 64) / 8) ^ (at_row & 7));
   pieces[(2 * h) * per + slot] = pack16<__half>(hi);
   if (second) pieces[(2 * h + 1) * per + slot] = pack16<__half>(lo);
 }
@@ -415,15 +461,14 @@ __global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* cou
 // so that the second finds the logits in the L2 cache).  Warp roles, each a loop over the items of the CTA:
 //   0      copies the blocks of the counts' pieces into the ring
 //   1      issues the products of a stage: three of 128 x columns x 64, into one of two accumulators
-//   2..9   epilogue, a thread per token and half of the columns: probabilities p_h from the logits, with the accumulator's row
-//   10..17 make the stage's two pieces of p_(1-h), 128 x 64 each, from the logits
+//   2..5   epilogue, a warp for 32 tokens: probabilities p_h from the logits, with the accumulator
+//   6..13  make the stage's two pieces of p_(1-h), 128 x 64 each, from the logits
 // Both kinds of readers of the logits have the next ones on the way while they work on the present ones.
 // Every wait is bounded; one that runs out raises FMOE_STATUS_WAIT_TIMEOUT and the CTA drains and leaves.
-constexpr int kMakers = 8, kReaders = 8;  // warps
+constexpr int kMakers = 8, kReaders = 4;  // warps
 constexpr int kProductThreads = (2 + kReaders + kMakers) * 32;
 constexpr int kPieceBytes = kTileTokens * 128;  // one piece of the probabilities
 constexpr int kMaxStages = 4;
-constexpr int kTurnPieces = 32 * 5;  // shared memory of a reading warp, in 16-byte pieces
 
 // a stage of the ring and the parity of its use
 struct RingCursor {
@@ -587,99 +632,146 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
   } else if (warp < 2 + kReaders) {
     bool ok = true;
     uint32_t round = 0;
-    const int quarter = warp & 3;     // the lanes of tensor memory that this warp may read
-    const int side = (warp - 2) / 4;  // the half of the columns
-    // 64 bytes of 32 rows at a time.  Memory is read and written with four lanes on a row, eight lines to an instruction; a
-    // thread per row would touch 32.  The chunk changes hands in shared memory, rows 80 bytes apart.
-    constexpr int N = Vec16<T>::N, kColumns = 4 * N;
-    uint4* turn = reinterpret_cast<uint4*>(gen + a.stages * stage_bytes) + (warp - 2) * kTurnPieces;
+    const int quarter = warp & 3;  // the lanes of tensor memory that this warp may read
+    // 32 rows x 32 columns at a time.  A thread has eight neighbouring columns, 8 (lane % 4) on, of the rows lane / 4 + 8 r in
+    // tensor memory as in global memory: nothing changes hands, and an instruction touches eight lines, where a thread per row would
+    // touch 32.
+    constexpr int N = Vec16<T>::N, kLoads = 8 / N, kRows = 4;
     const int64_t stride = 8 * a.ts, out_stride = 16 * static_cast<int64_t>(a.nk);
     const float unscale = a.head->unscale;
     const float scale = BACKWARD ? static_cast<float>(a.head->coef * static_cast<double>(*a.upstream)) : 0.f;
+    // what an item's tokens are read with; two chunks of logits are on the way, the next item's behind this one's
+    struct Source {
+      const T* rows;
+      int left;       // columns from the thread's first to the row's end
+      unsigned live;  // a bit a row
+    };
+    struct Stats {
+      float top[kRows], inv[kRows], s[kRows];
+    };
+    auto stats_of = [&](int i, Stats& w) {
+      const Item it = item_of(i);
+      const int64_t first = it.t0 + quarter * 32 + (lane >> 2);
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) {
+        const bool in = i < a.items && first + 8 * r < a.ntok;
+        w.top[r] = w.inv[r] = w.s[r] = 0.f;
+        load_if(in, reinterpret_cast<const float*>(a.stats + first + 8 * r) + 2 * it.h, w.top[r], w.inv[r]);
+        if (BACKWARD) load_if(in, a.token_s + first + 8 * r, w.s[r]);
+      }
+      if (BACKWARD && a.partials > 1) {  // calls of few tokens alone: no hurry
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+          if (i < a.items && first + 8 * r < a.ntok)
+            for (int c = 1; c < a.partials; ++c) w.s[r] += a.token_s[static_cast<int64_t>(c) * a.ntok + first + 8 * r];
+      }
+    };
+    auto source_of = [&](int i, const Stats& w) {
+      const Item it = item_of(i);
+      Source f;
+      const int ahead = it.n0 + (lane & 3) * 8;
+      f.rows = static_cast<const T*>(a.logits) + (it.t0 + quarter * 32 + (lane >> 2)) * a.ts + it.h * a.hs + ahead;
+      f.left = a.nk - ahead;
+      f.live = 0;
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) f.live |= w.inv[r] != 0.f ? 1u << r : 0u;
+      return f;
+    };
+    auto fetch = [&](const Source& f, int r, int c, uint4 (&to)[kLoads]) {
+      const T* at = f.rows + r * stride + c;
+#pragma unroll
+      for (int k = 0; k < kLoads; ++k) to[k] = load_piece<T, VEC>(at, k * N, f.left - c, (f.live >> r & 1u) != 0);
+    };
+    uint4 q[2][kRows][kLoads];
+    Stats stats;
+    stats_of(blockIdx.x, stats);
+    Source now = source_of(blockIdx.x, stats);
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+      fetch(now, r, 0, q[0][r]);
+      fetch(now, r, 32, q[1][r]);
+    }
     for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x, ++round) {
       const Item it = item_of(i);
       const uint32_t acc = round & 1u;
-      const int64_t t = it.t0 + quarter * 32 + lane;
-      const int c0 = side * (it.columns / 2), c1 = c0 + it.columns / 2;  // multiples of 32
-      float top = 0.f, inv = 0.f, s = 0.f;
-      if (t < a.ntok) {
-        const float4 st = a.stats[t];
-        top = it.h == 0 ? st.x : st.z;
-        inv = it.h == 0 ? st.y : st.w;
-      }
-      const float weight = BACKWARD ? (inv != 0.f ? inv * scale : 0.f) : inv * unscale;
-      // the lane's part of a chunk in memory: piece lane % 4 of the rows lane / 4 + 8 u
       const int64_t first = it.t0 + quarter * 32 + (lane >> 2);
-      const int ahead = it.n0 + (lane & 3) * N;
-      const T* rows = static_cast<const T*>(a.logits) + first * a.ts + it.h * a.hs + ahead;
-      T* outs = BACKWARD ? static_cast<T*>(a.dlogits) + (first * 2 + it.h) * a.nk + ahead : nullptr;
-      const int left = a.nk - ahead;  // columns from the lane's piece of the first chunk to the row's end
-      bool live[4];
+      T* outs = BACKWARD ? static_cast<T*>(a.dlogits) + (first * 2 + it.h) * a.nk + it.n0 + (lane & 3) * 8 : nullptr;
+      const int left = now.left;
+      // p (G - s) scale = e (acc weight + sum)
+      RowExp exp_of[kRows];
+      float weight[kRows], sum[kRows];
 #pragma unroll
-      for (int u = 0; u < 4; ++u) live[u] = __shfl_sync(kFull, inv, (lane >> 2) + 8 * u) != 0.f;
-      uint4 q[4];
-      auto fetch = [&](int c) {
-        const T* at = rows + c;
-#pragma unroll
-        for (int u = 0; u < 4; ++u, at += stride) q[u] = load_piece<T, VEC>(at, 0, left - c, live[u]);
-      };
-      fetch(c0);
-      if (BACKWARD && t < a.ntok)
-        for (int c = 0; c < a.partials; ++c) s += a.token_s[static_cast<int64_t>(c) * a.ntok + t];
+      for (int r = 0; r < kRows; ++r) {
+        const float inv = stats.inv[r];
+        exp_of[r] = RowExp(stats.top[r]);
+        weight[r] = inv * unscale;
+        sum[r] = 0.f;
+        if (BACKWARD) {
+          weight[r] = inv != 0.f ? inv * scale : 0.f;
+          sum[r] = -stats.s[r] * weight[r];
+          weight[r] *= unscale;
+        }
+      }
+      stats_of(i + gridDim.x, stats);
       ok = wait(tfull_bar(acc), (round >> 1) & 1u);
       if (!ok) break;
       ptx::tc_fence_after();
       const uint32_t taddr = tmem + acc * kChunk + (static_cast<uint32_t>(quarter * 32) << 16);
-      for (int c = c0; c < c1; c += kColumns) {
-#pragma unroll
-        for (int u = 0; u < 4; ++u) turn[((lane >> 2) + 8 * u) * 5 + (lane & 3)] = q[u];
-        __syncwarp();
-        if (c + kColumns < c1) fetch(c + kColumns);
-        uint32_t r[kColumns];
-        if constexpr (kColumns == 32) {
-          ptx::tmem_ld_32x32(taddr + c, r);
-        } else {
-          ptx::tmem_ld_32x16(taddr + c, r);
-        }
-        float p[4][N];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          unpack16<T>(turn[lane * 5 + v], p[v]);
-#pragma unroll
-          for (int k = 0; k < N; ++k) p[v][k] = exp_below(p[v][k] - top);
-        }
-        if constexpr (kColumns == 32) {
-          ptx::tmem_ld_wait(r);
-        } else {
-          ptx::tmem_ld_wait(r);
+      for (int c = 0; c < it.columns; c += 64) {
+        int to = c + 64;
+        if (to == it.columns) {  // the next item's first two chunks
+          to = 0;
+          now = source_of(i + gridDim.x, stats);
         }
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
+        for (int chunk = 0; chunk < 2; ++chunk)
 #pragma unroll
-          for (int k = 0; k < N; ++k) {
-            const float g = __uint_as_float(r[v * N + k]);
-            if (BACKWARD) p[v][k] = p[v][k] * fmaf(g, unscale, -s) * weight;
-            else s = fmaf(p[v][k], g, s);
+          for (int half = 0; half < 2; ++half) {
+            uint32_t g[16];
+            ptx::tmem_ld_32x256(taddr + (static_cast<uint32_t>(16 * half) << 16) + c + 32 * chunk, g);
+            float p[2][8];
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int r = 2 * half + u;
+#pragma unroll
+              for (int k = 0; k < kLoads; ++k) unpack16<T>(q[chunk][r][k], *reinterpret_cast<float (*)[N]>(&p[u][k * N]));
+              fetch(now, r, to + 32 * chunk, q[chunk][r]);
+#pragma unroll
+              for (int k = 0; k < 8; ++k) p[u][k] = exp_of[r](p[u][k]);
+            }
+            ptx::tmem_ld_wait(g);
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+              const int r = 2 * half + u;
+#pragma unroll
+              for (int k = 0; k < 8; ++k) {
+                const float v = __uint_as_float(g[4 * (k >> 1) + 2 * u + (k & 1)]);
+                if (BACKWARD) p[u][k] *= fmaf(v, weight[r], sum[r]);
+                else sum[r] = fmaf(p[u][k], v, sum[r]);
+              }
+              if (BACKWARD && first + 8 * r < a.ntok) {
+#pragma unroll
+                for (int k = 0; k < kLoads; ++k)
+                  store_piece<T, VEC>(outs + r * out_stride + c + 32 * chunk, k * N, left - c - 32 * chunk,
+                                      pack16<T>(*reinterpret_cast<float (*)[N]>(&p[u][k * N])));
+              }
+            }
           }
-          if (BACKWARD) turn[lane * 5 + v] = pack16<T>(p[v]);  // the lane's own row: nobody else reads it before the barrier
-        }
-        __syncwarp();
-        if (BACKWARD) {
-          T* out = outs + c;
-#pragma unroll
-          for (int u = 0; u < 4; ++u, out += out_stride)
-            if (first + 8 * u < a.ntok) store_piece<T, VEC>(out, 0, left - c, turn[((lane >> 2) + 8 * u) * 5 + (lane & 3)]);
-          __syncwarp();
-        }
       }
       ptx::tc_fence_before();
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(tempty_bar(acc));
       if (!BACKWARD) {
-        s *= weight;
-        if (t < a.ntok) a.token_s[static_cast<int64_t>(2 * it.chunk + side) * a.ntok + t] = s;
-        double all = s;
-        for (int d = 16; d > 0; d >>= 1) all += __shfl_xor_sync(kFull, all, d);
+        double all = 0.0;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+          sum[r] += __shfl_xor_sync(kFull, sum[r], 1);
+          sum[r] += __shfl_xor_sync(kFull, sum[r], 2);
+          sum[r] *= weight[r];
+          if ((lane & 3) == 0 && first + 8 * r < a.ntok) a.token_s[static_cast<int64_t>(it.chunk) * a.ntok + first + 8 * r] = sum[r];
+          all += sum[r];
+        }
+        for (int d = 16; d > 2; d >>= 1) all += __shfl_xor_sync(kFull, all, d);
         if (lane == 0) a.part[static_cast<int64_t>(i) * kReaders + warp - 2] = all;
       }
     }
@@ -704,11 +796,8 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
 #pragma unroll
       for (int r = 0; r < kRows; ++r) {
         w.top[r] = w.inv[r] = 0.f;
-        if (i < a.items && t0 + r * kStep < a.ntok) {
-          const float4 st = a.stats[t0 + r * kStep];
-          w.top[r] = it.h == 0 ? st.z : st.x;
-          w.inv[r] = it.h == 0 ? st.w : st.y;
-        }
+        load_if(i < a.items && t0 + r * kStep < a.ntok, reinterpret_cast<const float*>(a.stats + t0 + r * kStep) + 2 * (1 - it.h),
+                w.top[r], w.inv[r]);
       }
     };
     const int64_t stride = kStep * a.ts;
@@ -724,6 +813,9 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
     fetch(0, now);
     for (int i = blockIdx.x; i < a.items && ok; i += gridDim.x) {
       tokens(i + gridDim.x, next);
+      RowExp exp_of[kRows];
+#pragma unroll
+      for (int r = 0; r < kRows; ++r) exp_of[r] = RowExp(now.top[r]);
       for (int kb = 0; kb < blocks; ++kb, ring.next(a.stages)) {
         float p[kRows][8];
 #pragma unroll
@@ -732,7 +824,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
 #pragma unroll
           for (int k = 0; k < kLoads; ++k) unpack16<T>(x[r][k], *reinterpret_cast<float (*)[N]>(&p[r][k * N]));
 #pragma unroll
-          for (int k = 0; k < 8; ++k) p[r][k] = exp_below(p[r][k] - now.top[r]) * weight;
+          for (int k = 0; k < 8; ++k) p[r][k] = exp_of[r](p[r][k]) * weight;
         }
         if (kb + 1 < blocks) fetch(kb + 1, now);
         else fetch(0, next);
@@ -806,8 +898,8 @@ int item_width(int64_t T, int nk, int halves) {
   return width;
 }
 int chunks_of(int nk, int width) { return (padded_keys(nk) + width - 1) / width; }
-// what the forward leaves of s_t: a sum for each half of an item's columns
-int partial_sums(int64_t T, int nk) { return 2 * chunks_of(nk, item_width(T, nk, 1)); }
+// what the forward leaves of s_t: a sum for each item's columns
+int partial_sums(int64_t T, int nk) { return chunks_of(nk, item_width(T, nk, 1)); }
 
 template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStream_t stream) {
   const bool vec = vector_rows<T>(a) && (!BACKWARD || aligned16(a.dlogits));
@@ -815,9 +907,9 @@ template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStrea
   a.chunks = chunks_of(a.nk, a.width);
   a.partials = partial_sums(a.ntok, a.nk);
   const int stage = 2 * kPieceBytes + 2 * a.width * 128;
-  a.stages = 200 * 1024 / stage;
+  a.stages = 224 * 1024 / stage;
   if (a.stages > kMaxStages) a.stages = kMaxStages;
-  const int smem = a.stages * stage + kReaders * kTurnPieces * 16 + 1024;
+  const int smem = a.stages * stage + 1024;
   const int64_t items = token_tiles(a.ntok) * a.chunks * (BACKWARD ? 2 : 1);
   if (items > 0x7FFFFFFF / kReaders - 65536) return FMOE_ERR_UNSUPPORTED;
   a.items = static_cast<int>(items);
@@ -926,7 +1018,7 @@ size_t balance_prepared_bytes(int nk) { return nk <= 0 || nk > kMaxKeys ? 0 : kH
 size_t balance_stats_floats(int64_t T, int nk) { return T <= 0 || nk <= 0 || nk > kMaxKeys ? 0 : static_cast<size_t>(T) * (4 + partial_sums(T, nk)); }
 size_t balance_workspace_bytes(int64_t T, int nk) {
   if (T < 0 || nk <= 0 || nk > kMaxKeys) return 0;
-  return kParts * sizeof(Part) + static_cast<size_t>(token_tiles(T)) * (partial_sums(T, nk) / 2) * kReaders * sizeof(double);
+  return kParts * sizeof(Part) + static_cast<size_t>(token_tiles(T)) * partial_sums(T, nk) * kReaders * sizeof(double);
 }
 
 int launch_balance_forward(const void* logits, int64_t ts, int64_t hs, int dtype, const int64_t* counts, const uint8_t* mask, int64_t T,

@@ -167,6 +167,17 @@ __device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16])
       : "r"(taddr)
       : "memory");
 }
+// 256 bits of a lane for 32 threads, four times (shape 16x256b.x4): 16 lanes x 32 consecutive 32-bit columns, where thread i gets
+// of lane i / 4 and of lane i / 4 + 8 the columns 8 j + 2 (i % 4) and the next, j = 0..3: r[4 j], r[4 j + 1] and r[4 j + 2], r[4 j + 3].
+__device__ __forceinline__ void tmem_ld_32x256(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 // The registers of a tmem_ld are written some time before this wait ends, and the compiler takes them for written at the load:
 // it may move arithmetic on them, or a copy of them, in front of a wait that does not name them.  So the wait names them, and no
 // load is in flight where a loop closes, at which the compiler places such copies.

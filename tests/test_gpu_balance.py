@@ -109,8 +109,9 @@ def reference(logits, counts, mask, upstream):
     if not total or not tokens:
         return 0.0, 0.0, dlogits, slack
     p = torch.softmax(rows, -1)
-    every = p[0][:, :, None] * p[1][:, None, :]  # [tokens, nk, nk]
-    loss = nk * nk * ((c / total) * every.mean(0)).sum()
+    loss = 0.0
+    for part in p.split(max(1, (1 << 27) // (nk * nk)), 1):  # [tokens, nk, nk] at a time
+        loss = loss + nk * nk * ((c / total) * (part[0][:, :, None] * part[1][:, None, :]).sum(0)).sum() / tokens
     (grad,) = torch.autograd.grad(loss, rows, torch.tensor(upstream, dtype=torch.float64, device="cuda"))
     dlogits[:, keep] = grad
     p = p.detach()
@@ -158,6 +159,13 @@ SIZES = [(1, 1, 1), (1, 8, 4), (2, 3, 2), (5, 16, 4), (130, 32, 8), (500, 64, 16
 def test_loss_and_gradient(T, nk, k, dtype):
     # float16: a loss scale keeps the gradients, about 1 / (T nk), out of the subnormal numbers
     check(T, nk, k, dtype, seed=T, upstream=float(2 ** round(math.log2(T * nk))) if dtype == torch.float16 else 0.01)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,nk,k", [(60001, 16, 4), (40000, 64, 8), (38017, 100, 5), (45000, 192, 3)])
+def test_many_tokens(T, nk, k, dtype):
+    """Where two CTAs share the counts; masked tokens among them, and the last pair of CTAs with few or none."""
+    check(T, nk, k, dtype, masked=0.1, seed=T, upstream=float(2 ** round(math.log2(T * nk))) if dtype == torch.float16 else 1.0)
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
