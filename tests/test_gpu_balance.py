@@ -164,7 +164,7 @@ def test_loss_and_gradient(T, nk, k, dtype):
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,nk,k", [(60001, 16, 4), (40000, 64, 8), (38017, 100, 5), (45000, 192, 3)])
 def test_many_tokens(T, nk, k, dtype):
-    """Where two CTAs share the counts; masked tokens among them, and the last pair of CTAs with few or none."""
+    """Several items for every SM, masked tokens among them, and a last item with few or no tokens."""
     check(T, nk, k, dtype, masked=0.1, seed=T, upstream=float(2 ** round(math.log2(T * nk))) if dtype == torch.float16 else 1.0)
 
 
