@@ -209,48 +209,124 @@ template <typename T> __device__ __forceinline__ uint32_t minus_infinity() { ret
 template <> __device__ __forceinline__ uint32_t minus_infinity<__nv_bfloat16>() { return 0xFF80FF80u; }
 template <> __device__ __forceinline__ uint32_t minus_infinity<__half>() { return 0xFC00FC00u; }
 
-// the larger of each pair of values of two pieces; the other one where one is a NaN
-template <typename T> __device__ __forceinline__ uint4 piece_max(const uint4& a, const uint4& b) {
-  uint32_t x[4] = {a.x, a.y, a.z, a.w}, y[4] = {b.x, b.y, b.z, b.w};
+// A piece of a row: 8 or 4 logits, 16 bytes, from a column on, by loads of W bytes: 16 where rows are made of aligned pieces, 8 or 4
+// where they are made of such, and 2 for an odd number of 16-bit keys, where every other row starts in the middle of a word: there
+// the words that hold the piece are read, five of them, and shifted.  What lies behind the row's end, or in a row that is not
+// read, is minus infinity: its exponential is 0 and no use of the values has to ask.  Each load is one predicated instruction into
+// the register that holds the fill: with a branch, the compiler may copy the value where the ways meet, and a copy waits for it.
+template <typename T, int W> struct Piece {
+  static constexpr int N = Vec16<T>::N;
+  static constexpr int kRegs = W == 2 ? 6 : 4;
+  uint32_t w[kRegs];  // W = 2: five words, and 2 * columns to the row's end + whether the piece starts in the middle of the first
+  __device__ __forceinline__ void load(const T* at, int left, bool read) {  // `left` columns to the row's end
+    const uint32_t none = minus_infinity<T>();
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (sizeof(T) == 4) {
-      x[i] = __float_as_uint(fmaxf(__uint_as_float(x[i]), __uint_as_float(y[i])));
+    for (int i = 0; i < kRegs; ++i) w[i] = none;
+    if constexpr (W == 16) {
+      asm volatile(
+          "{\n\t"
+          ".reg .pred p;\n\t"
+          "setp.ne.s32 p, %5, 0;\n\t"
+          "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t"
+          "}\n"
+          : "+r"(w[0]), "+r"(w[1]), "+r"(w[2]), "+r"(w[3])
+          : "l"(__cvta_generic_to_global(at)), "r"(static_cast<int>(read && left > 0)));
+    } else if constexpr (W == 8) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.s32 p, %3, 0;\n\t"
+            "@p ld.global.v2.u32 {%0, %1}, [%2];\n\t"
+            "}\n"
+            : "+r"(w[2 * i]), "+r"(w[2 * i + 1])
+            : "l"(__cvta_generic_to_global(at + i * (N / 2))), "r"(static_cast<int>(read && left > i * (N / 2))));
     } else {
-      using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
-      const T2 m = __hmax2(*reinterpret_cast<const T2*>(&x[i]), *reinterpret_cast<const T2*>(&y[i]));
-      x[i] = *reinterpret_cast<const uint32_t*>(&m);
+      const char* from = reinterpret_cast<const char*>(at);
+      int odd = 0;
+      if (W == 2) {
+        odd = static_cast<int>(reinterpret_cast<uintptr_t>(at) >> 1) & 1;
+        from -= 2 * odd;  // an aligned word that holds a value of the row
+        w[kRegs - 1] = static_cast<uint32_t>((left > 0 && read ? left : 0) * 2 + odd);
+      }
+#pragma unroll
+      for (int i = 0; i < (W == 2 ? 5 : 4); ++i) {
+        bool in = read && left > i * (N / 4) - odd;
+        if (W == 2) in = in && left > 0 && i * 2 - odd < 8;
+        asm volatile(
+            "{\n\t"
+            ".reg .pred p;\n\t"
+            "setp.ne.s32 p, %2, 0;\n\t"
+            "@p ld.global.u32 %0, [%1];\n\t"
+            "}\n"
+            : "+r"(w[i])
+            : "l"(__cvta_generic_to_global(from + 4 * i)), "r"(static_cast<int>(in)));
+      }
     }
   }
-  return make_uint4(x[0], x[1], x[2], x[3]);
+  __device__ __forceinline__ void get(float* f) const {
+    uint4 q = make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (W == 2) {
+      if (w[5] & 1u)
+        q = make_uint4(__funnelshift_r(w[0], w[1], 16), __funnelshift_r(w[1], w[2], 16), __funnelshift_r(w[2], w[3], 16),
+                       __funnelshift_r(w[3], w[4], 16));
+    }
+    unpack16<T>(q, *reinterpret_cast<float (*)[N]>(f));
+    if constexpr (W == 2) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (i >= static_cast<int>(w[5] >> 1)) f[i] = -INFINITY;
+    }
+  }
+  // the larger of each two values; the other one where one is a NaN
+  __device__ __forceinline__ void join_max(const Piece& o) {
+    static_assert(W != 2, "its words are not values yet");
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        w[i] = __float_as_uint(fmaxf(__uint_as_float(w[i]), __uint_as_float(o.w[i])));
+      } else {
+        using T2 = std::conditional_t<std::is_same<T, __half>::value, __half2, __nv_bfloat162>;
+        const T2 m = __hmax2(*reinterpret_cast<const T2*>(&w[i]), *reinterpret_cast<const T2*>(&o.w[i]));
+        w[i] = *reinterpret_cast<const uint32_t*>(&m);
+      }
+    }
+  }
+};
+template <typename T, int W> __device__ __forceinline__ void store_values(T* at, int left, const float* f) {
+  constexpr int N = Vec16<T>::N;
+  const uint4 q = pack16<T>(*reinterpret_cast<const float (*)[N]>(f));
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if constexpr (W == 16) {
+    if (left > 0) *reinterpret_cast<uint4*>(at) = q;
+  } else if constexpr (W == 8) {
+    if (left > 0) *reinterpret_cast<uint2*>(at) = make_uint2(q.x, q.y);
+    if (left > N / 2) *reinterpret_cast<uint2*>(at + N / 2) = make_uint2(q.z, q.w);
+  } else if constexpr (W == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (left > i * (N / 4)) *reinterpret_cast<uint32_t*>(at + i * (N / 4)) = w[i];
+  } else {
+    uint16_t* p = reinterpret_cast<uint16_t*>(at);
+    const bool odd = (reinterpret_cast<uintptr_t>(at) & 2u) != 0;
+    if (left >= N && odd) {  // a value, three words, a value
+      p[0] = static_cast<uint16_t>(w[0]);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<uint32_t*>(p + 2 * i + 1) = __funnelshift_r(w[i], w[i + 1], 16);
+      p[7] = static_cast<uint16_t>(w[3] >> 16);
+    } else if (left >= N) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) *reinterpret_cast<uint32_t*>(p + 2 * i) = w[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (left > i) p[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+    }
+  }
 }
 
-// Pieces of a row: 16 bytes, 8 or 4 logits, from column c on.  What lies behind the row's end, or in a row that is not read, is
-// minus infinity: its exponential is 0 and no use of the values has to ask.  VEC: rows are made of aligned pieces.
-template <typename T, bool VEC> __device__ __forceinline__ uint4 load_piece(const T* row, int c, int nk, bool read = true) {
-  constexpr int N = Vec16<T>::N;
-  const uint32_t none = minus_infinity<T>();
-  uint4 q = make_uint4(none, none, none, none);
-  if constexpr (VEC) {
-    // one predicated load into the registers that hold the fill: with a branch, the compiler may copy the value where the ways
-    // meet, and a copy waits for it
-    asm volatile(
-        "{\n\t"
-        ".reg .pred p;\n\t"
-        "setp.ne.s32 p, %5, 0;\n\t"
-        "@p ld.global.v4.u32 {%0, %1, %2, %3}, [%4];\n\t"
-        "}\n"
-        : "+r"(q.x), "+r"(q.y), "+r"(q.z), "+r"(q.w)
-        : "l"(__cvta_generic_to_global(row + c)), "r"(static_cast<int>(read && c < nk)));
-  } else {
-    T v[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = read && c + i < nk ? row[c + i] : from_f32<T>(-INFINITY);
-    memcpy(&q, v, 16);
-  }
-  return q;
-}
-// likewise: what is not read stays as it was
+// such loads of one and two values: what is not read stays as it was
 __device__ __forceinline__ void load_if(bool read, const float* at, float& x, float& y) {
   asm volatile(
       "{\n\t"
@@ -271,23 +347,10 @@ __device__ __forceinline__ void load_if(bool read, const float* at, float& x) {
       : "+f"(x)
       : "l"(__cvta_generic_to_global(at)), "r"(static_cast<int>(read)));
 }
-template <typename T, bool VEC> __device__ __forceinline__ void store_piece(T* row, int c, int nk, const uint4& q) {
-  constexpr int N = Vec16<T>::N;
-  if constexpr (VEC) {
-    if (c < nk) *reinterpret_cast<uint4*>(row + c) = q;
-  } else {
-    T v[N];
-    memcpy(v, &q, 16);
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (c + i < nk) row[c + i] = v[i];
-  }
-}
-
 // (maximum, 1 / sum of exp(x - maximum)) of each half; 0, 0 for masked tokens, which are not read: no sum has an inverse of 0
 // Eight lanes share a row, so a warp has four tokens at a time and a lane enough values for its part of the reductions.  HELD: the
 // 16-byte pieces that a lane holds of each half; what longer rows have beside them is read again for the sum.
-template <typename T, bool VEC, int HELD>
+template <typename T, int W, int HELD>
 __global__ void __launch_bounds__(256, 4) balance_stats_kernel(const T* logits, int64_t ts, int64_t hs, const uint8_t* mask, int64_t ntok,
                                                             int nk, float4* stats, const int64_t* counts, Part* part) {
   pdl_launch_dependents();
@@ -335,25 +398,45 @@ __global__ void __launch_bounds__(256, 4) balance_stats_kernel(const T* logits, 
     const int64_t t = t0 + (lane >> 3);
     const bool live = ahead;
     const T* row[2] = {logits + t * ts, logits + t * ts + hs};
-    uint4 q[2][HELD];
+    Piece<T, W> q[2][HELD];
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int u = 0; u < HELD; ++u) q[h][u] = load_piece<T, VEC>(row[h], (u * 8 + sub) * N, nk, live);
+      for (int u = 0; u < HELD; ++u) q[h][u].load(row[h] + (u * 8 + sub) * N, nk - (u * 8 + sub) * N, live);
     ahead = reads(t + step);
     float top[2], sum[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      uint4 m = q[h][0];
-#pragma unroll
-      for (int u = 1; u < HELD; ++u) m = piece_max<T>(m, q[h][u]);
-      if (live)
-        for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) m = piece_max<T>(m, load_piece<T, VEC>(row[h], c, nk));
       float f[N];
-      unpack16<T>(m, f);
-      top[h] = f[0];
+      top[h] = -INFINITY;
+      if constexpr (W == 2) {
+        auto join = [&](const Piece<T, W>& v) {
+          v.get(f);
 #pragma unroll
-      for (int i = 1; i < N; ++i) top[h] = fmaxf(top[h], f[i]);
+          for (int i = 0; i < N; ++i) top[h] = fmaxf(top[h], f[i]);
+        };
+#pragma unroll
+        for (int u = 0; u < HELD; ++u) join(q[h][u]);
+        if (live)
+          for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) {
+            Piece<T, W> v;
+            v.load(row[h] + c, nk - c, true);
+            join(v);
+          }
+      } else {
+        Piece<T, W> m = q[h][0];
+#pragma unroll
+        for (int u = 1; u < HELD; ++u) m.join_max(q[h][u]);
+        if (live)
+          for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) {
+            Piece<T, W> v;
+            v.load(row[h] + c, nk - c, true);
+            m.join_max(v);
+          }
+        m.get(f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) top[h] = fmaxf(top[h], f[i]);
+      }
     }
 #pragma unroll
     for (int d = 4; d > 0; d >>= 1) {
@@ -364,16 +447,20 @@ __global__ void __launch_bounds__(256, 4) balance_stats_kernel(const T* logits, 
     for (int h = 0; h < 2; ++h) {
       float part[4] = {0.f, 0.f, 0.f, 0.f};
       const RowExp exp_of(top[h]);
-      auto join = [&](const uint4& v) {
+      auto join = [&](const Piece<T, W>& v) {
         float f[N];
-        unpack16<T>(v, f);
+        v.get(f);
 #pragma unroll
         for (int i = 0; i < N; ++i) part[i & 3] += exp_of(f[i]);
       };
 #pragma unroll
       for (int u = 0; u < HELD; ++u) join(q[h][u]);
       if (live)
-        for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) join(load_piece<T, VEC>(row[h], c, nk));
+        for (int c = (HELD * 8 + sub) * N; c < nk; c += 8 * N) {
+          Piece<T, W> v;
+          v.load(row[h] + c, nk - c, true);
+          join(v);
+        }
       sum[h] = (part[0] + part[1]) + (part[2] + part[3]);
     }
 #pragma unroll
@@ -506,7 +593,7 @@ __device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_
                : "memory");
 }
 
-template <typename T, bool VEC, bool BACKWARD>
+template <typename T, int W, bool BACKWARD>
 __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(const ProductArgs a) {
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bars[3 * kMaxStages + 4];
@@ -677,12 +764,12 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
       for (int r = 0; r < kRows; ++r) f.live |= w.inv[r] != 0.f ? 1u << r : 0u;
       return f;
     };
-    auto fetch = [&](const Source& f, int r, int c, uint4 (&to)[kLoads]) {
+    auto fetch = [&](const Source& f, int r, int c, Piece<T, W> (&to)[kLoads]) {
       const T* at = f.rows + r * stride + c;
 #pragma unroll
-      for (int k = 0; k < kLoads; ++k) to[k] = load_piece<T, VEC>(at, k * N, f.left - c, (f.live >> r & 1u) != 0);
+      for (int k = 0; k < kLoads; ++k) to[k].load(at + k * N, f.left - c - k * N, (f.live >> r & 1u) != 0);
     };
-    uint4 q[2][kRows][kLoads];
+    Piece<T, W> q[2][kRows][kLoads];
     Stats stats;
     stats_of(blockIdx.x, stats);
     Source now = source_of(blockIdx.x, stats);
@@ -734,7 +821,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
             for (int u = 0; u < 2; ++u) {
               const int r = 2 * half + u;
 #pragma unroll
-              for (int k = 0; k < kLoads; ++k) unpack16<T>(q[chunk][r][k], *reinterpret_cast<float (*)[N]>(&p[u][k * N]));
+              for (int k = 0; k < kLoads; ++k) q[chunk][r][k].get(&p[u][k * N]);
               fetch(now, r, to + 32 * chunk, q[chunk][r]);
 #pragma unroll
               for (int k = 0; k < 8; ++k) p[u][k] = exp_of[r](p[u][k]);
@@ -752,8 +839,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
               if (BACKWARD && first + 8 * r < a.ntok) {
 #pragma unroll
                 for (int k = 0; k < kLoads; ++k)
-                  store_piece<T, VEC>(outs + r * out_stride + c + 32 * chunk, k * N, left - c - 32 * chunk,
-                                      pack16<T>(*reinterpret_cast<float (*)[N]>(&p[u][k * N])));
+                  store_values<T, W>(outs + r * out_stride + c + 32 * chunk + k * N, left - c - 32 * chunk - k * N, &p[u][k * N]);
               }
             }
           }
@@ -788,7 +874,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
       float top[kRows], inv[kRows];
     };
     Rows now, next;
-    uint4 x[kRows][kLoads];
+    Piece<T, W> x[kRows][kLoads];
     auto tokens = [&](int i, Rows& w) {
       const Item it = item_of(i);
       const int64_t t0 = it.t0 + r0;
@@ -807,7 +893,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
 #pragma unroll
       for (int r = 0; r < kRows; ++r, at += stride)
 #pragma unroll
-        for (int k = 0; k < kLoads; ++k) x[r][k] = load_piece<T, VEC>(at, k * N, left, w.inv[r] != 0.f);
+        for (int k = 0; k < kLoads; ++k) x[r][k].load(at + k * N, left - k * N, w.inv[r] != 0.f);
     };
     tokens(blockIdx.x, now);
     fetch(0, now);
@@ -822,7 +908,7 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
         for (int r = 0; r < kRows; ++r) {
           const float weight = now.inv[r] * 32768.f;
 #pragma unroll
-          for (int k = 0; k < kLoads; ++k) unpack16<T>(x[r][k], *reinterpret_cast<float (*)[N]>(&p[r][k * N]));
+          for (int k = 0; k < kLoads; ++k) x[r][k].get(&p[r][k * N]);
 #pragma unroll
           for (int k = 0; k < 8; ++k) p[r][k] = exp_of[r](p[r][k]) * weight;
         }
@@ -882,10 +968,11 @@ __global__ void __launch_bounds__(kProductThreads, 1) balance_product_kernel(con
 size_t matrix_bytes(int nk) { return static_cast<size_t>(padded_keys(nk)) * padded_keys(nk) * 2; }
 int64_t token_tiles(int64_t T) { return (T + kTileTokens - 1) / kTileTokens; }
 
-// rows made of aligned 16-byte pieces
-template <typename T> bool vector_rows(const ProductArgs& a) {
-  constexpr int V = Vec16<T>::N;
-  return a.nk % V == 0 && a.ts % V == 0 && a.hs % V == 0 && aligned16(a.logits);
+// bytes of the loads that rows of these sizes and addresses allow: 16, 8, 4 or, for 16-bit types, 2
+template <typename T> int load_width(const ProductArgs& a, const void* out) {
+  const uintptr_t bits = (static_cast<uintptr_t>(a.nk) | static_cast<uintptr_t>(a.ts) | static_cast<uintptr_t>(a.hs)) * sizeof(T) |
+                         reinterpret_cast<uintptr_t>(a.logits) | reinterpret_cast<uintptr_t>(out);
+  return bits % 16 == 0 ? 16 : bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : 2;
 }
 
 // Columns of an item: as few as 64 while the items still fit the SMs side by side, since an item's latency is what small calls
@@ -902,7 +989,7 @@ int chunks_of(int nk, int width) { return (padded_keys(nk) + width - 1) / width;
 int partial_sums(int64_t T, int nk) { return chunks_of(nk, item_width(T, nk, 1)); }
 
 template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStream_t stream) {
-  const bool vec = vector_rows<T>(a) && (!BACKWARD || aligned16(a.dlogits));
+  const int bytes = load_width<T>(a, a.dlogits);
   a.width = item_width(a.ntok, a.nk, BACKWARD ? 2 : 1);
   a.chunks = chunks_of(a.nk, a.width);
   a.partials = partial_sums(a.ntok, a.nk);
@@ -919,7 +1006,11 @@ template <typename T, bool BACKWARD> int launch_product(ProductArgs a, cudaStrea
     FMOE_CUDA_TRY(launch_pdl(BACKWARD ? 0 : 32, kern, dim3(grid), dim3(kProductThreads), smem, stream, 1, a));
     return FMOE_OK;
   };
-  return vec ? run(balance_product_kernel<T, true, BACKWARD>) : run(balance_product_kernel<T, false, BACKWARD>);
+  if (bytes == 16) return run(balance_product_kernel<T, 16, BACKWARD>);
+  if (bytes == 8) return run(balance_product_kernel<T, 8, BACKWARD>);
+  if constexpr (sizeof(T) == 2)
+    if (bytes == 2) return run(balance_product_kernel<T, 2, BACKWARD>);
+  return run(balance_product_kernel<T, 4, BACKWARD>);
 }
 
 template <typename T>
@@ -927,10 +1018,12 @@ int forward_typed(ProductArgs a, const uint8_t* mask, const int64_t* counts, Pre
   const int64_t want = (a.ntok + 31) / 32, cap = static_cast<int64_t>(device_sm_count()) * 16;
   const int64_t grid = want > cap ? cap : want < kParts ? kParts : want;
   constexpr int kLine = 8 * Vec16<T>::N;  // columns of eight lanes' pieces
-  auto* kern = !vector_rows<T>(a) ? (a.nk <= 2 * kLine ? balance_stats_kernel<T, false, 2> : balance_stats_kernel<T, false, 4>)
-               : a.nk <= kLine    ? balance_stats_kernel<T, true, 1>
-               : a.nk <= 2 * kLine ? balance_stats_kernel<T, true, 2>
-                                   : balance_stats_kernel<T, true, 4>;
+  const int bytes = load_width<T>(a, nullptr);
+  auto* kern = a.nk <= kLine ? balance_stats_kernel<T, 16, 1> : a.nk <= 2 * kLine ? balance_stats_kernel<T, 16, 2> : balance_stats_kernel<T, 16, 4>;
+  if (bytes == 8) kern = a.nk <= 2 * kLine ? balance_stats_kernel<T, 8, 2> : balance_stats_kernel<T, 8, 4>;
+  if (bytes == 4) kern = a.nk <= 2 * kLine ? balance_stats_kernel<T, 4, 2> : balance_stats_kernel<T, 4, 4>;
+  if constexpr (sizeof(T) == 2)
+    if (bytes == 2) kern = a.nk <= 2 * kLine ? balance_stats_kernel<T, 2, 2> : balance_stats_kernel<T, 2, 4>;
   kern<<<static_cast<unsigned>(grid), 256, 0, stream>>>(static_cast<const T*>(a.logits), a.ts, a.hs, mask, a.ntok, a.nk, stats, counts, part);
   FMOE_LAUNCH_CHECK();
   const int64_t pieces = static_cast<int64_t>(a.padded) * a.padded / 4;
