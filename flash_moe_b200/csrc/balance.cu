@@ -118,7 +118,8 @@ __global__ void __launch_bounds__(kCountThreads) expert_counts_kernel(const int6
 
 // Many selections of not too many experts: every CTA counts all its selections in shared memory, in 16 bits an expert, and the
 // eight CTAs of a cluster add theirs up before they go to global memory, each a part of the experts and in ascending order.
-// At 4.2 million selections of 65536 experts the tables above are mostly taken by others: 30 us, by this kernel 21.
+// At 4.2 million selections of 65536 experts the tables above are mostly taken by others.  What is left of its 21 us there is
+// 34 MB of ids (5 us), the atomics in shared memory and 120 CTAs' worth of counters on their way to global memory.
 constexpr int kHistCtas = 8;
 constexpr int kHistThreads = 1024;
 constexpr int kHistExperts = 102400;      // 200 KB
@@ -977,11 +978,13 @@ template <typename T> int load_width(const ProductArgs& a, const void* out) {
 
 // Columns of an item: as few as 64 while the items still fit the SMs side by side, since an item's latency is what small calls
 // cost; each item makes the probabilities of its tokens again.
+// The number of SMs is that of a B200 whatever the device has: what the forward leaves of s_t depends on the width.
+constexpr int kSideBySide = 148;
 int item_width(int64_t T, int nk, int halves) {
   const int padded = padded_keys(nk);
   int width = padded < kChunk ? padded : kChunk;
   for (int w = 64; w < width; w *= 2)
-    if (token_tiles(T) * ((padded + w - 1) / w) * halves <= device_sm_count()) width = w;
+    if (token_tiles(T) * ((padded + w - 1) / w) * halves <= kSideBySide) return w;
   return width;
 }
 int chunks_of(int nk, int width) { return (padded_keys(nk) + width - 1) / width; }
@@ -1094,10 +1097,11 @@ int launch_expert_counts(const int64_t* indices, const uint8_t* mask, int64_t T,
     return launch_cluster(expert_counts_kernel<true>, ctas, kCountThreads, ctas, 0, stream, indices, mask, pairs, k, N, out, status);
   }
   FMOE_CUDA_TRY(cudaMemsetAsync(counts, 0, static_cast<size_t>(N) * 8, stream));
-  if (pairs >= (1 << 20) && N <= kHistExperts && pairs >= 16 * N) {
+  // measured, whole call, Zipf exponent 0.7, tables and histogram: 16384 experts, 262144 selections 10.4 and 12.1 us, 1048576 17.8 and
+  // 13.6; 65536 experts, 1048576 selections 17.7 and 17.7, 4194304 32.1 and 22.0; 256 experts, 524288 selections 13.8 and 9.9
+  const int clusters = pairs >= (1 << 19) && N <= kHistExperts && pairs >= 32 * N ? histogram_clusters() : 0;
+  if (clusters > 0) {
     const int smem = static_cast<int>((N + 7) / 8) * 16;
-    const int clusters = histogram_clusters();
-    if (clusters <= 0) return FMOE_ERR_UNSUPPORTED;
     return launch_cluster(expert_histogram_kernel, clusters * kHistCtas, kHistThreads, kHistCtas, smem, stream, indices, mask, pairs, k,
                           static_cast<int>(N), out, status);
   }

@@ -9,7 +9,7 @@ usual pre-norm decoder block.  `GraphedFlashMoE(stack, x)` captures the whole st
 
 `fused_norm=True` (with `pre_norm`) takes skip connection and norm between two layers of a training step in one kernel each way
 (`add_rms_norm`) instead of torch's addition and rms_norm; the sums are rounded alike, the normalised values and gradients agree
-to within their rounding.  `balance_loss` and `clip_grad_norm_` are what a training step needs beside the layers."""
+to within their rounding (under autocast, or with norm weights of another dtype, torch's functions stay).  `balance_loss` and `clip_grad_norm_` are what a training step needs beside the layers."""
 
 from __future__ import annotations
 
@@ -43,7 +43,8 @@ class FlashMoEStack(nn.Module):
     def forward(self, hidden_states: torch.Tensor, return_routing: bool = False) -> Tuple[torch.Tensor, List[torch.Tensor]]:
         """Returns the final hidden states and every layer's router logits.  ``return_routing=True`` keeps every layer's
         selected ids and gates in its ``last_indices`` / ``last_gates``."""
-        if self.norms is not None and self.fused_norm and torch.is_grad_enabled() \
+        if self.norms is not None and self.fused_norm and torch.is_grad_enabled() and not torch.is_autocast_enabled("cuda") \
+                and all(w.dtype == hidden_states.dtype for w in self.norms) \
                 and (hidden_states.requires_grad or any(p.requires_grad for p in self.parameters())):
             return self._forward_fused_norm(hidden_states, return_routing)
         all_logits = []

@@ -98,7 +98,8 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
     residual and weight; x, residual and weight share one dtype, up to 16384 columns."""
     eps = float(eps)
     if plain_call():
-        return _forward(x, residual, weight, eps)
+        normed, summed = _forward(x, residual, weight, eps)
+        return normed, x if residual is None else summed
     if residual is None:
         return AddRMSNormFunc.apply(x, None, weight, eps), x
     return AddRMSNormFunc.apply(x, residual, weight, eps)
@@ -117,10 +118,11 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor] = None, w
     if group_size not in (None, 32, 64, 128):
         raise _lib.FmoeError("group_size must be None, 32, 64 or 128")
     eps = float(eps)
+    given = x
     dev, x, r, w, rows, H = _arguments(x, residual, weight, eps)
     q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
     scales = x.new_empty((*x.shape[:-1], 1 if group_size is None else -(-H // group_size)), dtype=torch.float32)
-    summed = x if r is None else torch.empty_like(x)
+    summed = given if r is None else torch.empty_like(x)
     rc = _lib.call("fmoe_add_rms_norm_fp8", dev, x.data_ptr(), _lib.ptr(r), _lib.ptr(w), None if r is None else summed.data_ptr(),
                    q.data_ptr(), scales.data_ptr(), _lib.dtype_code(x), rows, H, group_size or 0, eps)
     if rc:

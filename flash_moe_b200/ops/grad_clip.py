@@ -101,6 +101,7 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     are left out, one given twice counts once.  float32, bfloat16 and float16 gradients may be mixed; each must be dense, and all on
     one device."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
+    max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0:
         raise _lib.FmoeError("max_norm and eps must not be negative")
     grads = _once([g for g in [p.grad for p in parameters] if g is not None],
