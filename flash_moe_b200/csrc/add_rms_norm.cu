@@ -20,7 +20,7 @@ constexpr unsigned kFull = 0xFFFFFFFFu;
 constexpr float kE4m3Max = 448.f;
 constexpr float kMinScale = 1.17549435e-38f;  // 2^-126: a zero group keeps a scale that can be divided by
 
-// VEC values of T as they are loaded: 16 bytes, or one value where rows are not made of aligned 16-byte pieces
+// VEC values of T as they are loaded: 16 bytes, or one value where an array does not start at a multiple of 16 bytes
 template <typename T, int VEC> struct Piece {
   uint4 q;
   __device__ __forceinline__ void load(const T* p) { q = ld16(p); }

@@ -5,9 +5,8 @@
 // Memory-bound: every gradient is read once for the norm and, only where the factor is not 1, read and written once more.
 // One launch covers up to kTensors tensors: their addresses travel as a kernel parameter, nothing is copied to the device.  The
 // chunks of all tensors form one list of which each CTA has a contiguous piece, so the sums are formed in a fixed order.
-#include <cstdlib>
-#include <new>
 #include <algorithm>
+#include <new>
 
 #include "common.cuh"
 
@@ -83,8 +82,11 @@ template <typename T> __device__ __forceinline__ float chunk_squares(const Walk&
   }
   const T* p = reinterpret_cast<const T*>(w.at);
   for (int e = w.rest(sizeof(T)); e < static_cast<int>(w.bytes / sizeof(T)); e += kThreads) {
-    const float f = to_f32<T>(p[e]);
-    acc[0] = fmaf(f, f, acc[0]);
+    const float f = to_f32<T>(p[e]), oldest = acc[0];  // the four sums in turn: as short as those of whole pieces
+    acc[0] = acc[1];
+    acc[1] = acc[2];
+    acc[2] = acc[3];
+    acc[3] = fmaf(f, f, oldest);
   }
   return (acc[0] + acc[1]) + (acc[2] + acc[3]);
 }

@@ -9,7 +9,8 @@ usual pre-norm decoder block.  `GraphedFlashMoE(stack, x)` captures the whole st
 
 `fused_norm=True` (with `pre_norm`) takes skip connection and norm between two layers of a training step in one kernel each way
 (`add_rms_norm`) instead of torch's addition and rms_norm; the sums are rounded alike, the normalised values and gradients agree
-to within their rounding (under autocast, or with norm weights of another dtype, torch's functions stay).  `balance_loss` and `clip_grad_norm_` are what a training step needs beside the layers."""
+to within their rounding.  Under autocast, or with norm weights of another dtype, torch's functions stay.  `balance_loss` and
+`clip_grad_norm_` are what a training step needs beside the layers."""
 
 from __future__ import annotations
 

@@ -226,6 +226,18 @@ def test_strides_alignment_and_leading_dimensions(dtype):
     assert torch.equal(a, b)
 
 
+def test_without_a_residual_the_sum_is_x_itself():
+    from flash_moe_b200 import add_rms_norm, add_rms_norm_fp8
+
+    x = torch.randn(40, 64, device="cuda").t()  # not contiguous
+    with torch.no_grad():
+        assert add_rms_norm(x)[1] is x
+        assert add_rms_norm_fp8(x)[2] is x
+    leaf = x.clone().requires_grad_(True)
+    normed, summed = add_rms_norm(leaf)
+    assert summed is leaf and torch.equal(normed, add_rms_norm(x)[0])
+
+
 def test_no_rows():
     from flash_moe_b200 import add_rms_norm, add_rms_norm_fp8
 

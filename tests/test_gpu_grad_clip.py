@@ -1,9 +1,10 @@
 """`grad_norm` and `clip_grad_norm_` against the formulas in 64 bits.
 
-u = 2^-24 is half a step of float32.  A piece of 16 KiB is summed in float32: each thread has at most 32 squares in four chains
-(8 products and additions each: 9 u), two more additions, a warp's and CTA's sums in float64; so the sum of squares is off by
-at most 12 u and the norm by half of that and two roundings: 8 u.  The factor adds three roundings (12 u in all), its product
-with a gradient one more and the rounding to the gradient's type."""
+u = 2^-24 is half a step of float32.  A piece of 32 KiB is summed in float32 by 256 threads: a thread has at most 64 squares of
+16-bit values (32 of float32) in four chains of 16, and one value of a ragged end more; each is one fused step with one rounding,
+all terms are positive, two additions join the chains: 16 + 1 + 2 = 19 u on the sum, all further sums are in float64.  The root
+halves that and is rounded once to float32: 10.5 u, so 11 u on the norm.  The factor adds a sum, a quotient and a product (14 u in
+all), its product with a gradient one more (15 u), and then comes the rounding to the gradient's type."""
 
 import math
 
@@ -40,10 +41,10 @@ def check(params, max_norm, scale=1.0, **more):
     norm, grads = expected(params, max_norm, scale)
     got = clip_grad_norm_(params, max_norm, **more)
     assert got.shape == () and got.dtype == torch.float32
-    assert abs(float(got) - norm) <= 8 * U * norm
+    assert abs(float(got) - norm) <= 11 * U * norm
     for p, want in zip(params, grads):
         fi = torch.finfo(p.dtype)
-        bound = want.abs() * (fi.eps / 2 * (1 + 14 * U) + 14 * U) + fi.tiny * fi.eps
+        bound = want.abs() * (fi.eps / 2 * (1 + 15 * U) + 15 * U) + fi.tiny * fi.eps
         assert bool(((p.grad.double() - want).abs() <= bound).all())
     return float(got)
 
@@ -110,7 +111,7 @@ def test_gradients_given_twice_count_once():
     twin = torch.nn.Parameter(torch.zeros(100, device="cuda"))
     twin.grad = params[0].grad
     got = clip_grad_norm_([*params, params[0], twin], 1.0)
-    assert abs(float(got) - norm) <= 8 * U * norm
+    assert abs(float(got) - norm) <= 11 * U * norm
     assert torch.allclose(params[0].grad.double(), grads[0], rtol=16 * U, atol=0)
 
 
@@ -155,12 +156,12 @@ def test_norm_alone():
     params = gradients(SHAPES, DTYPES, seed=12)
     norm, _ = expected(params, 1.0)
     before = [p.grad.clone() for p in params]
-    assert abs(float(grad_norm([p.grad for p in params])) - norm) <= 8 * U * norm
-    assert abs(float(grad_norm([p.grad for p in params], 0.5)) - norm / 2) <= 8 * U * norm
+    assert abs(float(grad_norm([p.grad for p in params])) - norm) <= 11 * U * norm
+    assert abs(float(grad_norm([p.grad for p in params], 0.5)) - norm / 2) <= 11 * U * norm
     assert all(torch.equal(p.grad, b) for p, b in zip(params, before))
     gaps = params[-1].grad[:, ::2]
     want = math.sqrt(float(gaps.double().square().sum()))
-    assert abs(float(grad_norm(gaps)) - want) <= 8 * U * want
+    assert abs(float(grad_norm(gaps)) - want) <= 11 * U * want
 
 
 def test_refusals():

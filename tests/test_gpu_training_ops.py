@@ -81,6 +81,27 @@ def test_fused_norm_changes_training_alone():
     assert torch.equal(ya, yb) and all(torch.equal(p, q) for p, q in zip(la, lb))
 
 
+def test_fused_norm_under_autocast_and_mixed_types():
+    """Torch's norm stays where the norm's weights have another type than the states and where autocast chooses the types: the same
+    bits as without `fused_norm`."""
+    x, _, _ = data()
+    a, b = make_stack(True), make_stack(False)
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        ya, yb = a(x)[0], b(x)[0]
+    assert ya.dtype == yb.dtype and torch.equal(ya, yb)
+    a, b = make_stack(True, torch.bfloat16), make_stack(False, torch.bfloat16)
+    for stack in (a, b):
+        stack.norms[1].data = stack.norms[1].data.float()
+    outcomes = []
+    for stack in (a, b):
+        try:
+            outcomes.append(stack(x.bfloat16())[0])
+        except (RuntimeError, ValueError) as e:
+            outcomes.append(str(e))
+    assert type(outcomes[0]) is type(outcomes[1])
+    assert outcomes[0] == outcomes[1] if isinstance(outcomes[0], str) else torch.equal(*outcomes)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_training_step_in_16_bits_runs(dtype):
     """Every gradient is there and finite, and the norm is the one of the clipped gradients."""
