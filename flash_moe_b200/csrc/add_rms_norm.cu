@@ -705,6 +705,7 @@ int launch_add_rms_norm_backward(const void* dnormed, const void* dsummed, const
   }
   if (dnormed == nullptr || summed == nullptr || dx == nullptr) return FMOE_ERR_BAD_ARG;
   if (dweight != nullptr && (ws == nullptr || ws_bytes < add_rms_norm_backward_workspace_bytes(rows, H, dtype))) return FMOE_ERR_WORKSPACE;
+  if (dweight != nullptr && !aligned16(ws)) return FMOE_ERR_ALIGNMENT;
   float* part = static_cast<float*>(ws);
   switch (dtype) {
     case FMOE_DTYPE_F32: return backward_typed<float>(dnormed, dsummed, summed, weight, dx, dweight, part, rows, H, eps, stream);

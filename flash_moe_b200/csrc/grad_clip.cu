@@ -6,6 +6,7 @@
 // One launch covers up to kTensors tensors: their addresses travel as a kernel parameter, nothing is copied to the device.  The
 // chunks of all tensors form one list of which each CTA has a contiguous piece, so the sums are formed in a fixed order.
 #include <algorithm>
+#include <cfloat>
 #include <new>
 
 #include "common.cuh"
@@ -239,12 +240,13 @@ int launch_grad_norm(void* const* grads, const int64_t* numels, const int32_t* d
                      float eps, float scale, const float* device_scale, float* norm, void* ws, size_t ws_bytes,
                      cudaStream_t stream) {
   if (count < 0 || norm == nullptr || (count > 0 && (grads == nullptr || numels == nullptr || dtypes == nullptr))) return FMOE_ERR_BAD_ARG;
-  if (!(scale >= 0.f) || (clip && (!(max_norm >= 0.f) || !(eps >= 0.f)))) return FMOE_ERR_BAD_ARG;
+  if (!(scale >= 0.f && scale <= FLT_MAX) || (clip && (!(max_norm >= 0.f) || !(eps >= 0.f)))) return FMOE_ERR_BAD_ARG;
   if (count == 0) {
     FMOE_CUDA_TRY(cudaMemsetAsync(norm, 0, sizeof(float), stream));
     return FMOE_OK;
   }
   if (ws == nullptr || ws_bytes < grad_norm_workspace_bytes(count)) return FMOE_ERR_WORKSPACE;
+  if (!aligned16(ws)) return FMOE_ERR_ALIGNMENT;
   const int rc = check_tensors(grads, numels, dtypes, count);
   if (rc != FMOE_OK) return rc;
   double* part = static_cast<double*>(ws);

@@ -31,8 +31,8 @@ def _call(name, grads: List[torch.Tensor], head, grad_scale) -> torch.Tensor:
         if grad_scale.dtype != torch.float32 or grad_scale.numel() != 1 or grad_scale.device != dev:
             raise _lib.FmoeError("a grad_scale tensor must hold one float32 value on the device of the gradients")
         scale, device_scale = 1.0, grad_scale.data_ptr()
-    elif not 0 <= grad_scale < float("inf"):
-        raise _lib.FmoeError("grad_scale must be a finite number that is not negative")
+    elif not 0 <= grad_scale <= torch.finfo(torch.float32).max:
+        raise _lib.FmoeError("grad_scale must be a finite float32 number that is not negative")
     n = len(grads)
     try:
         codes = array("i", [_lib.DTYPE_CODE[g.dtype] for g in grads])
@@ -98,8 +98,9 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     With ``n = grad_scale * sqrt(sum of all squares)`` every gradient is multiplied by ``grad_scale * min(1, max_norm / (n + eps))``
     in float32 and rounded once; where that factor is 1 nothing is written.  `grad_scale` is a number or one float32 on the device:
     the inverse of a loss scale, or the number of ranks where averaged gradients are to be summed.  Parameters without a gradient
-    are left out, one given twice counts once.  float32, bfloat16 and float16 gradients may be mixed; each must be dense, and all on
-    one device."""
+    are left out, one given twice counts once.  float32, bfloat16 and float16 gradients may be mixed; each must be dense, all on
+    one device, and no two may share a part of their memory.  The norm is that of the gradients given: ranks that hold different
+    parameters combine their `grad_norm`s first."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0:

@@ -207,7 +207,8 @@ int fmoe_rms_norm(const void* x, const void* weight, void* out, int dtype, int64
  *                               each row (group 0) or each `group` = 32, 64 or 128 columns of it ([T, ceil(H / group)], the last
  *                               block may be short), q [T, H] = e4m3(y / scale).  A value that is not finite makes its scale so
  *   fmoe_add_rms_norm_backward  from dnormed and dsummed (nullable) the gradient dx of both x and residual, and dweight
- *                               (nullable): sums in float32 in a fixed order, one rounding
+ *                               (nullable): sums in float32 in a fixed order, one rounding; the workspace, 16-byte
+ *                               aligned, is for dweight
  * residual (nullable, then summed is null too: x itself is normalised), weight (nullable) [hidden].  hidden is any number up to
  * 16384, arrays may start anywhere; where they all start at 16 bytes, rows of any length are read in aligned pieces of that size.
  */
@@ -227,7 +228,8 @@ int fmoe_add_rms_norm_backward(const void* dnormed, const void* dsummed, const v
  *                        factor is 1.  A norm that is not finite makes the gradients so, or zero them, as the formula says
  * grads, numels and dtypes are HOST arrays of num_tensors entries, grads device pointers to dense tensors of any alignment, no
  * two of which may share memory.  scale >= 0; device_scale (nullable, one float in device memory) multiplies it: the inverse of
- * a loss scale.  Squares and products in float32, the sum over 32 KiB pieces in float64, in a fixed order.
+ * a loss scale.  Squares and products in float32, the sum over 32 KiB pieces in float64, in a fixed order.  The workspace is
+ * 16-byte aligned.
  */
 size_t fmoe_grad_norm_workspace_bytes(int num_tensors);
 int fmoe_grad_norm(void* const* grads, const int64_t* numels, const int32_t* dtypes, int num_tensors, float scale,

@@ -238,6 +238,21 @@ def test_without_a_residual_the_sum_is_x_itself():
     assert summed is leaf and torch.equal(normed, add_rms_norm(x)[0])
 
 
+def test_x_as_its_own_residual():
+    """s = x + x is exact, and so is the sum of the two equal gradients.  The other call has a residual too, of zeros: without one the
+    sum is x itself, whose gradient autograd adds to the rounded one of the norm, one rounding more than the fused gradient has."""
+    from flash_moe_b200 import add_rms_norm
+
+    x = torch.randn(9, 72, device="cuda").bfloat16().requires_grad_(True)
+    normed, summed = add_rms_norm(x, x)
+    doubled = (2 * x.detach()).requires_grad_(True)
+    normed_of, summed_of = add_rms_norm(doubled, torch.zeros_like(doubled))
+    assert torch.equal(summed, doubled) and torch.equal(normed, normed_of)
+    up = torch.randn_like(normed)
+    (got,), (half,) = torch.autograd.grad((normed, summed), x, (up, up)), torch.autograd.grad((normed_of, summed_of), doubled, (up, up))
+    assert torch.equal(got, 2 * half)
+
+
 def test_no_rows():
     from flash_moe_b200 import add_rms_norm, add_rms_norm_fp8
 

@@ -168,6 +168,27 @@ def test_many_tokens(T, nk, k, dtype):
     check(T, nk, k, dtype, masked=0.1, seed=T, upstream=float(2 ** round(math.log2(T * nk))) if dtype == torch.float16 else 1.0)
 
 
+def test_offsets_beyond_32_bits():
+    """2^31 logits and a few rows more.  With the number of rows as the upstream gradient a row's gradient is that of any batch with
+    its own number; it is compared by the bounds of the formula, not with another call, whose sums of 64 columns are others: where
+    G - s cancels, two right results differ by more than a step of their type."""
+    from flash_moe_b200 import balance_loss, expert_counts
+
+    nk, rows, tail = 512, 2**31 // 1024 + 200, 200
+    g = torch.Generator(device="cuda").manual_seed(2)
+    counts = expert_counts(torch.randint(0, nk * nk // 7, (4096, 32), device="cuda", generator=g), nk * nk)
+    tile = torch.randn(128, 2, nk, device="cuda", generator=g).bfloat16()
+    flat = tile.new_empty(rows, 2, nk)
+    flat[: rows // 128 * 128].view(-1, 128, 2, nk).copy_(tile)
+    flat[rows // 128 * 128 :].copy_(tile[: rows % 128])
+    logits = flat.transpose(0, 1).requires_grad_(True)
+    (got,) = torch.autograd.grad(balance_loss(logits, counts), logits, torch.tensor(float(rows), device="cuda"))
+    for part in (slice(0, tail), slice(rows - tail, rows)):
+        _, _, want, slack = reference(logits.detach()[:, part], counts, None, float(tail))
+        bound = slack + (want.abs() + slack) * 2.0**-8 + torch.finfo(torch.bfloat16).tiny
+        assert bool(((got[:, part].double() - want).abs() <= bound).all())
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("T,nk,k", [(1, 8, 4), (100, 33, 5), (700, 64, 16)])
 def test_masked_tokens(T, nk, k, dtype):

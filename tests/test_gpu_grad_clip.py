@@ -169,6 +169,7 @@ def test_refusals():
 
     (p,) = gradients([(8, 8)], torch.float32)
     for max_norm, more in [(-1.0, {}), (float("nan"), {}), (1.0, dict(grad_scale=-1.0)), (1.0, dict(grad_scale=float("inf"))),
+                           (1.0, dict(grad_scale=1e39)),  # infinite as a float32
                            (1.0, dict(eps=-1.0)), (1.0, dict(grad_scale=torch.ones((), device="cuda", dtype=torch.float64))),
                            (1.0, dict(grad_scale=torch.ones(2, device="cuda"))), (1.0, dict(grad_scale=torch.ones(())))]:
         before = p.grad.clone()

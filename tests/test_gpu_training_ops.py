@@ -201,3 +201,81 @@ def test_serving_norm_between_layers():
         assert bool((off <= torch.maximum(xn.float().abs() * (2.0**-4 + 2.0**-7), scales * 2.0**-10 + 2.0**-8 * xn.float().abs())).all())
         out, _ = stack.layers[1](xn)
         assert out.shape == x.shape
+
+
+def tiled(tile, rows):
+    """`rows` rows that repeat those of `tile`."""
+    out = tile.new_empty((rows, *tile.shape[1:]))
+    whole = rows // len(tile) * len(tile)
+    out[:whole].view(-1, *tile.shape).copy_(tile)
+    out[whole:].copy_(tile[: rows - whole])
+    return out
+
+
+def test_norm_offsets_beyond_32_bits():
+    """2^31 values and a few rows more: the last rows are the bits of a small call."""
+    from flash_moe_b200 import add_rms_norm, add_rms_norm_fp8
+
+    H, tail = 1000, 5
+    rows = 2**31 // H + 100
+    g = torch.Generator(device="cuda").manual_seed(1)
+    tile = torch.randn(64, H, device="cuda", generator=g).bfloat16()
+    w = torch.randn(H, device="cuda", generator=g).bfloat16()
+    big = tiled(tile, rows)
+    last = big[-tail:].clone()
+    with torch.no_grad():
+        for got, want in zip(add_rms_norm(big, big, w), add_rms_norm(last, last, w)):
+            assert torch.equal(got[-tail:], want)
+        for got, want in zip(add_rms_norm_fp8(big, None, w, group_size=64), add_rms_norm_fp8(last, None, w, group_size=64)):
+            assert torch.equal(got[-tail:].float(), want.float())
+    del got
+    big.requires_grad_(True)
+    (dx,) = torch.autograd.grad(add_rms_norm(big, None, w)[0], big, big.detach())
+    small = last.requires_grad_(True)
+    (want,) = torch.autograd.grad(add_rms_norm(small, None, w)[0], small, small.detach())
+    assert torch.equal(dx[-tail:], want)
+
+
+def test_clip_offsets_beyond_32_bits():
+    from flash_moe_b200 import clip_grad_norm_
+
+    param = torch.nn.Parameter(torch.empty(2**31 + 1000, device="cuda", dtype=torch.bfloat16))
+    param.grad = torch.full_like(param, 2.0**-16)
+    param.grad[-1] = 1.0
+    norm = clip_grad_norm_(param, 0.5)
+    expected = (1.0 + (2**31 + 999) * 2.0**-32) ** 0.5
+    assert abs(float(norm) - expected) <= 2.0**-20 * expected  # 11 u are derived for any gradients: 2^-20.5
+    assert abs(float(param.grad[-1]) - 0.5 / expected) <= 2.0**-8 and bool((param.grad[-3:-1] == param.grad[0]).all())
+    assert abs(float(param.grad[0]) * 2.0**16 - 0.5 / expected) <= 2.0**-8
+
+
+def test_two_streams_at_once():
+    """Calls of every operator on two streams, not ordered against each other: each has the bits of a call alone."""
+    from flash_moe_b200 import add_rms_norm, balance_loss, clip_grad_norm_, expert_counts
+
+    def work(seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        x, r = (torch.randn(700, 512, device="cuda", generator=g) for _ in range(2))
+        logits = torch.randn(2, 900, 64, device="cuda", generator=g)
+        idx = torch.randint(0, 4096, (900, 8), device="cuda", generator=g)
+        return x, r, logits, idx
+
+    def run(x, r, logits, idx):
+        x, logits = x.clone().requires_grad_(True), logits.clone().requires_grad_(True)
+        n, s = add_rms_norm(x, r)
+        loss = balance_loss(logits, expert_counts(idx, 4096))
+        ((n * s).sum() + loss).backward()
+        return [n.detach(), s.detach(), loss.detach(), clip_grad_norm_([x, logits], 0.1), x.grad, logits.grad]
+
+    inputs = [work(s) for s in (1, 2)]
+    want = [run(*i) for i in inputs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream() for _ in range(2)], [[], []]
+    for _ in range(5):
+        for j, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[j].append(run(*inputs[j]))
+    torch.cuda.synchronize()
+    for j in range(2):
+        for outputs in got[j]:
+            assert all(torch.equal(a, b) for a, b in zip(outputs, want[j]))

@@ -44,6 +44,7 @@ def test_norm(lib):
     assert lib.fmoe_add_rms_norm_backward(*args, p(5), size - 1, None) == WORKSPACE
     assert lib.fmoe_add_rms_norm_backward(*args, None, size, None) == WORKSPACE
     assert lib.fmoe_add_rms_norm_backward(None, *args[1:], p(5), size, None) == BAD_ARG
+    assert lib.fmoe_add_rms_norm_backward(*args, ctypes.c_void_p(4098), size, None) == 4
     assert lib.fmoe_add_rms_norm_backward_workspace_bytes(0, 64, 1) == 0
 
 
@@ -89,6 +90,8 @@ def test_clip(lib):
     assert clip([4096], [8], [0], norm=None) == BAD_ARG and clip([None], [8], [0]) == BAD_ARG
     assert clip([4096], [-8], [0]) == BAD_ARG and clip([4096], [8], [3]) == BAD_ARG
     assert clip([4096], [8], [0], ws=None) == WORKSPACE and clip([4096], [8], [0], size=8) == WORKSPACE
+    assert clip([4096], [8], [0], scale=float("inf")) == BAD_ARG and clip([4096], [8], [0], scale=float("nan")) == BAD_ARG
+    assert clip([4096], [8], [0], ws=ctypes.c_void_p(4104)) == 4  # sums of 8 bytes, but the rule is 16
     assert clip([4098], [8], [0]) == 4  # a float32 between two others
     # memory that two tensors share, whatever their order
     assert clip([8192, 4096], [8, 1025], [0, 0]) == BAD_ARG and clip([4096, 4096], [8, 8], [1, 1]) == BAD_ARG
