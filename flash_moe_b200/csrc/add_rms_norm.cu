@@ -3,10 +3,11 @@
 // (flash_moe/modules/flash_moe.py:55-59).
 //
 // Memory-bound throughout: the forward moves 4 rows' worth of values per row (x, r in; s, n out), the backward 4 (dn, ds, s in;
-// dx out).  32768 x 2048 bfloat16 take 80 us forward and 85 + 4 backward (6.7 and 6.3 TB/s of 6.47 that a copy reaches), the 8-bit
-// form 42 us at 16384 x 2048 with blocks of 128 columns (5.6 TB/s; 71 % of the issue slots).  A row stays in the registers of its group of warps between the sum of squares and the scaling, so each value is
-// moved once.  Everything inside is float32; s is rounded to T before it is normalised, so that n belongs to the s that is
-// stored and the backward finds the same s; n, dx and dw are rounded once.
+// dx out).  32768 x 2048 bfloat16 take 80 us forward (6.7 TB/s, where a copy reaches 6.5) and 89 + 4 backward (6.0 TB/s), the
+// 8-bit form 42 us at 16384 x 2048 with blocks of 128 columns (5.6 TB/s; 71 % of the issue slots).  A row stays in the registers
+// of its group of warps between the sum of squares and the scaling, so each value is moved once.  Everything inside is float32; s
+// is rounded to T before it is normalised, so that n belongs to the s that is stored and the backward finds the same s; n, dx and
+// dw are rounded once.
 #include <cuda_fp8.h>
 
 #include <cstring>
