@@ -556,9 +556,10 @@ __global__ void __launch_bounds__(256) balance_prepare_kernel(const int64_t* cou
 // At 131072 tokens x 256 keys, bfloat16, it takes 50 us forward (134 MB of logits, 17 GF three times) and 93 us backward (268 MB, 34 GF
 // three times), the tensor pipe busy 55 % of the time in both.  In a program that measured parts of it the backward took 98 us, without
 // its epilogue's stores 82, without its epilogue 72, with nothing but the copies and the products 61: the warps that make and read
-// probabilities hide behind the products in part only.  Measured and not kept: pairs of CTAs that hold the counts' pieces in shared memory for all items (forward and
-// backward 102 us on average, this form 83 at the time: fewer stages are left for the probabilities), logits fetched two stages
-// ahead, streaming stores.  Small calls are a chain of latencies: 4096 x 128, 8 + 8 us.
+// probabilities hide behind the products in part only.  Measured and not kept: pairs of CTAs that hold the counts' pieces in shared
+// memory for all items (forward and backward 102 us on average, this form 83 at the time: fewer stages are left for the
+// probabilities), a second team of readers for every other item (backward 102 and 106 us with one and two chunks of logits on the
+// way), logits fetched two stages ahead, streaming stores.  Small calls are a chain of latencies: 4096 x 128, 8 + 8 us.
 // Every wait is bounded; one that runs out raises FMOE_STATUS_WAIT_TIMEOUT and the CTA drains and leaves.
 constexpr int kMakers = 8, kReaders = 4;  // warps
 constexpr int kProductThreads = (2 + kReaders + kMakers) * 32;
