@@ -111,7 +111,8 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor] = None, w
 
     ``quantised`` is float8_e4m3fn in the shape of x; ``scales`` is float32, ``[..., 1]`` for one scale a row (``group_size=None``)
     or ``[..., ceil(hidden / group_size)]`` for one scale for each 32, 64 or 128 columns: the largest absolute value of the row or
-    block / 448 (at least 2^-126).  The float32 value is rounded once, to 8 bits."""
+    block / 448 (at least 2^-126).  The float32 value is divided by its scale, by an approximate reciprocal (2^-21), and rounded once, to
+    8 bits."""
     if torch.is_grad_enabled() and (x.requires_grad or residual is not None and residual.requires_grad
                                     or weight is not None and weight.requires_grad):
         raise _lib.FmoeError("add_rms_norm_fp8 has no gradient: call it under torch.no_grad(), or add_rms_norm")

@@ -205,7 +205,10 @@ int fmoe_rms_norm(const void* x, const void* weight, void* out, int dtype, int64
  *   fmoe_add_rms_norm           summed = s, normed = dtype(s * rsqrt(mean(s^2) + eps) * weight)
  *   fmoe_add_rms_norm_fp8       summed = s, and the float32 value y of the norm in 8 bits: scales = max(max |y| / 448, 2^-126) over
  *                               each row (group 0) or each `group` = 32, 64 or 128 columns of it ([T, ceil(H / group)], the last
- *                               block may be short), q [T, H] = e4m3(y / scale).  A value that is not finite makes its scale so
+ *                               block may be short), q [T, H] = e4m3(y / scale).  The scale is a product with 1 / 448, within 2^-23
+ *                               of the quotient, and y / scale a product with an approximate reciprocal, within 2^-21: nearer than
+ *                               that to the middle between two values of 8 bits, q is either.  A value that is not finite makes
+ *                               its scale so
  *   fmoe_add_rms_norm_backward  from dnormed and dsummed (nullable) the gradient dx of both x and residual, and dweight
  *                               (nullable): sums in float32 in a fixed order, one rounding; the workspace, 16-byte
  *                               aligned, is for dweight

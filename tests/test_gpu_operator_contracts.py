@@ -1,0 +1,47 @@
+"""What the headers and docstrings of the norm, the clipping and the balance loss promise at the ends of their ranges: 8-bit
+quotients, rows shorter than a 16-byte piece, weights that start anywhere, tensors given twice, the widest rows of keys."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [None, 32, 64, 128])
+@pytest.mark.parametrize("H", [256, 512, 333, 2048, 8200])
+def test_fp8_quotients(H, group, dtype):
+    """scale = max |y| / 448 by a product with the rounded 1 / 448: 2^-24 for each of the two roundings, 2^-23 in all.  q = e4m3(y / scale)
+    by an approximate reciprocal of that scale, 2 ulp = 2^-22 of it, and a product, 2^-24: less than 2^-21 of the quotient, so q is
+    what one of the ends of that interval rounds to.
+
+    A row of +-1 has a mean square of 1 and is its own norm, so y is the weight, exactly.  The weights of a block are multiples of 1/448
+    of its largest, many of them in the middle between two values of 8 bits."""
+    from flash_moe_b200 import add_rms_norm, add_rms_norm_fp8
+
+    g = torch.Generator().manual_seed(H)
+    size = group or H
+    # odd multiples of 16: 5 bits, of which e4m3 keeps 4; the factor has what the type's bits leave
+    middles = torch.tensor([17.0, 19, 21, 23, 25, 27, 29, 31])[torch.randint(0, 8, (H,), generator=g)] * 2.0 ** torch.randint(-3, 4, (H,), generator=g)
+    middles[::size] = 448.0
+    bases = torch.randint(1, {torch.bfloat16: 4, torch.float16: 16}.get(dtype, 64), (-(-H // size),), generator=g) * 2.0 + 1
+    w = middles * bases.repeat_interleave(size)[:H] * 2.0**-9
+    assert torch.equal(w.to(dtype).float(), w)
+    if H % 2 == 0 and dtype is torch.float32:
+        w[1::2] = torch.randn(w[1::2].shape, generator=g)  # any bits at all
+    signs = torch.randint(0, 2, (6, H), generator=g) * 2.0 - 1
+    x, r, wd = ((signs * 0.25).to(dtype).cuda(), (signs * 0.75).to(dtype).cuda(), w.to(dtype).cuda())
+    with torch.no_grad():
+        normed, summed = add_rms_norm(x, r, None, 0.0)
+        assert torch.equal(summed.cpu().float(), signs) and torch.equal(normed, summed)
+        q, scales, _ = add_rms_norm_fp8(x, r, wd, 0.0, group)
+    y = (signs * w).double()
+    want = torch.nn.functional.pad(y.abs(), (0, -H % size)).view(6, -1, size).amax(-1) / 448
+    assert bool(((scales.cpu().double() - want).abs() <= want * 2.0**-23).all())
+    quotient = y / scales.cpu().double().repeat_interleave(size, 1)[:, :H]
+    # a float32 in between would round twice: the ends' last bits are set away from the quotient by more than they are rounded
+    ends = [(quotient * (1 + sign * 2.0**-21)).float().to(torch.float8_e4m3fn).float() for sign in (-1, 1)]
+    q = q.cpu().float()
+    assert bool(((q == ends[0]) | (q == ends[1])).all())
