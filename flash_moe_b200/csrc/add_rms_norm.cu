@@ -564,15 +564,12 @@ struct Shape {
 constexpr Shape kVecShapes[] = {FMOE_VEC_SHAPES(FMOE_SHAPE)};
 constexpr Shape kOneShapes[] = {FMOE_ONE_SHAPES(FMOE_SHAPE)};
 #undef FMOE_SHAPE
-int shape_of(bool vec, int pieces) {
+template <int N> int smallest_shape(const Shape (&shapes)[N], int pieces) {
   int i = 0;
-  if (vec) {
-    while (kVecShapes[i].wpg * 32 * kVecShapes[i].c < pieces) ++i;
-    return i;
-  }
-  while (kOneShapes[i].wpg * 32 * kOneShapes[i].c < pieces) ++i;
-  return i;
+  while (i < N && shapes[i].wpg * 32 * shapes[i].c < pieces) ++i;
+  return i;  // N, which no launch takes, where none holds that many
 }
+int shape_of(bool vec, int pieces) { return vec ? smallest_shape(kVecShapes, pieces) : smallest_shape(kOneShapes, pieces); }
 
 // Groups that the grid of a backward has: all that its registers let run at once, and no more, since each group leaves a row of
 // partial sums.  A multiple of eight, so that SHIFT keeps its remainders.
@@ -624,20 +621,21 @@ int launch_backward(const NormBackwardArgs<T>& in, T* dweight, cudaStream_t stre
 // kWhole: rows of aligned pieces; kShifted: rows of any length in memory that starts at a piece; kSingle: one value at a time
 enum Form { kWhole, kShifted, kSingle };
 constexpr int kMostPieces = 4096;  // of the widest shape
-// pieces of a row, at most
-int pieces_of(Form form, int vec, int H) { return form == kSingle ? H : form == kWhole ? H / vec : (H + 2 * vec - 2) / vec; }
-Form form_of(int vec, int H, std::initializer_list<const void*> pointers) {
+// pieces of a row, at most; rows of whole pieces have as many when their weights are read one by one (kShifted, no shift)
+int pieces_of(Form form, int vec, int H) { return form == kSingle ? H : H % vec == 0 ? H / vec : (H + 2 * vec - 2) / vec; }
+// kShifted reads weights one by one, so they may start anywhere
+Form form_of(int vec, int H, const void* weight, std::initializer_list<const void*> pointers) {
   for (const void* p : pointers)
     if (!aligned16(p)) return kSingle;
-  return H % vec == 0 ? kWhole : pieces_of(kShifted, vec, H) <= kMostPieces ? kShifted : kSingle;
+  if (H % vec == 0 && aligned16(weight)) return kWhole;
+  return pieces_of(kShifted, vec, H) <= kMostPieces ? kShifted : kSingle;
 }
 
 template <typename T>
 int forward_typed(const void* x, const void* residual, const void* weight, void* summed, void* normed, void* q, float* scales,
                   int64_t rows, int H, int group, float eps, int mode, cudaStream_t stream) {
   constexpr int V = Vec16<T>::N;
-  Form form = form_of(V, H, {x, residual, summed, normed, q});
-  if (form == kWhole && !aligned16(weight)) form = kShifted;  // which reads weights one by one
+  const Form form = form_of(V, H, weight, {x, residual, summed, normed, q});
   const NormArgs<T> a = {static_cast<const T*>(x), static_cast<const T*>(residual), static_cast<const T*>(weight),
                          static_cast<T*>(summed), static_cast<T*>(normed), static_cast<__nv_fp8_storage_t*>(q), scales, rows, H, 1,
                          group == 32 ? 5 : group == 64 ? 6 : 7, mode == kFp8Block ? (H + group - 1) / group : 1, eps};
@@ -657,8 +655,7 @@ template <typename T>
 int backward_typed(const void* dnormed, const void* dsummed, const void* summed, const void* weight, void* dx, void* dweight,
                    float* part, int64_t rows, int H, float eps, cudaStream_t stream) {
   constexpr int V = Vec16<T>::N;
-  Form form = form_of(V, H, {dnormed, dsummed, summed, dx});
-  if (form == kWhole && !aligned16(weight)) form = kShifted;
+  const Form form = form_of(V, H, weight, {dnormed, dsummed, summed, dx});
   const NormBackwardArgs<T> a = {static_cast<const T*>(dnormed), static_cast<const T*>(dsummed), static_cast<const T*>(summed),
                                  static_cast<const T*>(weight), static_cast<T*>(dx), dweight != nullptr ? part : nullptr, rows, H, 1, eps};
   T* dw = static_cast<T*>(dweight);

@@ -3,10 +3,9 @@ quotients, rows shorter than a 16-byte piece, weights that start anywhere, tenso
 
 import pytest
 import torch
+from test_gpu_add_rms_norm import DTYPES, EPS, U, inputs, near, randn, row_u, sum_and_norm
 
 pytestmark = pytest.mark.gpu
-
-DTYPES = [torch.float32, torch.bfloat16, torch.float16]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -45,3 +44,44 @@ def test_fp8_quotients(H, group, dtype):
     ends = [(quotient * (1 + sign * 2.0**-21)).float().to(torch.float8_e4m3fn).float() for sign in (-1, 1)]
     q = q.cpu().float()
     assert bool(((q == ends[0]) | (q == ends[1])).all())
+
+
+def check_norm(x, r, w, dn, ds):
+    """Forward, gradients and 8 bits against the formulas in 64 bits, within the bounds that test_gpu_add_rms_norm.py derives."""
+    from flash_moe_b200 import add_rms_norm, add_rms_norm_fp8
+
+    T, H = x.shape
+    x, r, w = (t.requires_grad_() for t in (x, r, w))
+    normed, summed = add_rms_norm(x, r, w, EPS)
+    dx, dr, dw = torch.autograd.grad((normed, summed), (x, r, w), (dn, ds))
+    normed, summed, x, r, w = (t.detach() for t in (normed, summed, x, r, w))
+    want, y = sum_and_norm(x, r, w)
+    assert torch.equal(summed, want) and torch.equal(dx, dr)
+    near(normed, y, y.abs() * row_u(H))
+    s, wd, dnd, dsd = summed.double(), w.double(), dn.double(), ds.double()
+    rstd = 1 / torch.sqrt(s.square().mean(-1, keepdim=True) + EPS)
+    g = dnd * wd
+    k, kabs = (rstd**2 * v.mean(-1, keepdim=True) for v in (g * s, (g * s).abs()))
+    near(dx, dsd + rstd * (g - s * k), 3 * row_u(H) * (dsd.abs() + rstd * (g.abs() + s.abs() * kabs)))
+    terms = dnd * s * rstd
+    near(dw, terms.sum(0), (row_u(H) + (T + 32) * U) * terms.abs().sum(0))
+    for group in (None, 32, 64):
+        size = group or H
+        blocks = -(-H // size)
+        q, scales, again = add_rms_norm_fp8(x, r, w, EPS, group)
+        assert torch.equal(again, summed) and scales.shape == (T, blocks)
+        top = torch.nn.functional.pad(y.abs(), (0, blocks * size - H)).view(T, blocks, size).amax(-1)
+        assert bool(((scales.double() - top / 448).abs() <= top / 448 * (row_u(H) + 2 * U)).all())
+        wide = scales.double().repeat_interleave(size, 1)[:, :H]
+        bound = torch.maximum(y.abs() * 2.0**-4, wide * 2.0**-10) + y.abs() * (row_u(H) + 8 * U)
+        assert bool(((q.double() * wide - y).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("H", [80, 512, 8192, 16384, 16380])
+def test_weights_that_start_anywhere(H, dtype):
+    """Rows of whole aligned pieces beside a weight that starts between two of them."""
+    x, r, w = inputs(3, H, dtype, seed=H)
+    odd = torch.empty(H + 1, device="cuda", dtype=dtype)[1:].copy_(w)
+    assert odd.data_ptr() % 16 != 0 and x.data_ptr() % 16 == 0
+    check_norm(x, r, odd, randn(3, H, seed=1, dtype=dtype), randn(3, H, seed=2, dtype=dtype))
