@@ -12,6 +12,7 @@
 
 #include <cstring>
 #include <initializer_list>
+#include <numeric>
 
 #include "common.cuh"
 
@@ -103,7 +104,8 @@ template <typename T, int VEC> __device__ __forceinline__ void keep_part(Piece<T
 // one, but rows r, r + VEC, r + 2 VEC, ... all at the same: with SHIFT a group takes the rows of one remainder, and its pieces are
 // the aligned ones of memory, of which a row's first and last lie in it in part.  A thread's columns, its weights and its part of
 // dweight are the same for every row then.  Pieces are read whole, with the neighbours' values, which `mask` takes out where they
-// are used (a wait inside the read would stop the reads behind it); only the last row's end is read value by value.
+// are used (a wait inside the read would stop the reads behind it); only the last row's end is read value by value, so rows are not
+// shorter than what a piece may reach into the next.
 template <int VEC, int WPG, bool SHIFT> struct Walk {
   int64_t row, step, rows;
   int H, shift, pieces;
@@ -623,12 +625,15 @@ enum Form { kWhole, kShifted, kSingle };
 constexpr int kMostPieces = 4096;  // of the widest shape
 // pieces of a row, at most; rows of whole pieces have as many when their weights are read one by one (kShifted, no shift)
 int pieces_of(Form form, int vec, int H) { return form == kSingle ? H : H % vec == 0 ? H / vec : (H + 2 * vec - 2) / vec; }
+// A row's last piece reaches into what follows by up to vec - gcd(H, vec) values.  The row behind it has to cover them: rows of 1, 2, 3
+// and 5 16-bit values, and of one float32, are too short.
+bool may_shift(int vec, int H) { return pieces_of(kShifted, vec, H) <= kMostPieces && vec - std::gcd(H, vec) <= H; }
 // kShifted reads weights one by one, so they may start anywhere
 Form form_of(int vec, int H, const void* weight, std::initializer_list<const void*> pointers) {
   for (const void* p : pointers)
     if (!aligned16(p)) return kSingle;
   if (H % vec == 0 && aligned16(weight)) return kWhole;
-  return pieces_of(kShifted, vec, H) <= kMostPieces ? kShifted : kSingle;
+  return may_shift(vec, H) ? kShifted : kSingle;
 }
 
 template <typename T>
@@ -697,7 +702,7 @@ size_t add_rms_norm_backward_workspace_bytes(int64_t rows, int H, int dtype) {
   const int n = 16 / dtype_size(dtype);
   int64_t groups = 0;
   for (const Form form : {kWhole, kShifted, kSingle}) {
-    if (form != kSingle && pieces_of(form, n, H) > kMostPieces) continue;
+    if (form != kSingle && !may_shift(n, H)) continue;  // H is at most kMostPieces whole ones, which may shift
     const Shape sh = form == kSingle ? kOneShapes[shape_of(false, H)] : kVecShapes[shape_of(true, pieces_of(form, n, H))];
     const int64_t g = backward_groups(sh, rows);
     groups = g > groups ? g : groups;
