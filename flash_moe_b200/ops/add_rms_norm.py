@@ -9,7 +9,7 @@ from typing import Optional, Tuple
 import torch
 
 from .. import _lib
-from .utils import backward_once, contiguous, plain_call
+from .utils import backward_once, contiguous, plain_call, plain_call_without_gradient
 
 MAX_HIDDEN = 16384
 
@@ -105,6 +105,27 @@ def add_rms_norm(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weigh
     return AddRMSNormFunc.apply(x, residual, weight, eps)
 
 
+def _forward_fp8(x, residual, weight, eps, group_size):
+    dev, x, r, w, rows, H = _arguments(x, residual, weight, eps)
+    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    scales = x.new_empty((*x.shape[:-1], 1 if group_size is None else -(-H // group_size)), dtype=torch.float32)
+    summed = x if r is None else torch.empty_like(x)
+    rc = _lib.call("fmoe_add_rms_norm_fp8", dev, x.data_ptr(), _lib.ptr(r), _lib.ptr(w), None if r is None else summed.data_ptr(),
+                   q.data_ptr(), scales.data_ptr(), _lib.dtype_code(x), rows, H, group_size or 0, eps)
+    if rc:
+        _lib.check(rc, "fmoe_add_rms_norm_fp8")
+    return q, scales, summed
+
+
+class AddRMSNormFP8Func(torch.autograd.Function):
+    """What refuses tangents and what a trace records; there is no gradient."""
+
+    @staticmethod
+    def forward(ctx, x, residual, weight, eps, group_size):
+        q, scales, summed = _forward_fp8(x, residual, weight, eps, group_size)
+        return (q, scales, summed) if residual is not None else (q, scales)
+
+
 def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None,
                      eps: float = 1e-6, group_size: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """``(quantised, scales, summed)``: the norm above in 8 bits, ``quantised * scales`` in its place (inference only).
@@ -119,13 +140,9 @@ def add_rms_norm_fp8(x: torch.Tensor, residual: Optional[torch.Tensor] = None, w
     if group_size not in (None, 32, 64, 128):
         raise _lib.FmoeError("group_size must be None, 32, 64 or 128")
     eps = float(eps)
-    given = x
-    dev, x, r, w, rows, H = _arguments(x, residual, weight, eps)
-    q = torch.empty_like(x, dtype=torch.float8_e4m3fn)
-    scales = x.new_empty((*x.shape[:-1], 1 if group_size is None else -(-H // group_size)), dtype=torch.float32)
-    summed = given if r is None else torch.empty_like(x)
-    rc = _lib.call("fmoe_add_rms_norm_fp8", dev, x.data_ptr(), _lib.ptr(r), _lib.ptr(w), None if r is None else summed.data_ptr(),
-                   q.data_ptr(), scales.data_ptr(), _lib.dtype_code(x), rows, H, group_size or 0, eps)
-    if rc:
-        _lib.check(rc, "fmoe_add_rms_norm_fp8")
-    return q, scales, summed
+    if plain_call_without_gradient():
+        q, scales, summed = _forward_fp8(x, residual, weight, eps, group_size)
+        return q, scales, x if residual is None else summed
+    if residual is None:
+        return (*AddRMSNormFP8Func.apply(x, None, weight, eps, group_size), x)
+    return AddRMSNormFP8Func.apply(x, residual, weight, eps, group_size)

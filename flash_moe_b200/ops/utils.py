@@ -21,6 +21,11 @@ def plain_call() -> bool:
     return not _grad_enabled() and forward_ad._current_level < 0 and not _tracing()
 
 
+def plain_call_without_gradient() -> bool:
+    """The same for an op that has no gradient, whatever the grad mode."""
+    return forward_ad._current_level < 0 and not _tracing()
+
+
 def backward_once(backward):
     """``once_differentiable`` for the backward of an op: a second differentiation is refused.  Where no graph of the backward is
     recorded, which is nearly always, its bookkeeping (4 us of host time) is left out."""

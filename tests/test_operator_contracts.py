@@ -1,0 +1,45 @@
+"""Contracts of the operators around the layer that need no GPU, with the library calls replaced."""
+
+import sys
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from flash_moe_b200 import add_rms_norm_fp8
+
+
+@pytest.fixture
+def fp8_without_a_gpu(monkeypatch):
+    """The op doubles its input, out of autograd's sight as the library does."""
+    def doubled(x, residual, weight, eps, group):
+        y = torch.from_numpy(2 * x.detach().numpy())
+        return y, torch.ones(x.shape[0], 1), y.clone()
+
+    norm = sys.modules["flash_moe_b200.ops.add_rms_norm"]
+    monkeypatch.setattr(norm, "_forward_fp8", doubled, raising=False)
+    monkeypatch.setattr(norm._lib, "require_cuda", lambda *t: t[0].device)
+    monkeypatch.setattr(norm._lib, "call", lambda name, *a: 0)
+
+
+@pytest.mark.parametrize("op", [lambda x: add_rms_norm_fp8(x), lambda x: add_rms_norm_fp8(x, x)])
+def test_tangents_are_refused_not_dropped(op, fp8_without_a_gpu):
+    with torch.no_grad(), forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="jvp"):
+            op(forward_ad.make_dual(torch.ones(2, 3), torch.ones(2, 3)))
+        assert torch.equal(op(torch.ones(2, 3))[0], torch.full((2, 3), 2.0))  # a level alone is no tangent
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning", "ignore::DeprecationWarning")
+@pytest.mark.parametrize("op", [lambda x: add_rms_norm_fp8(x)[0], lambda x: add_rms_norm_fp8(x, x)[2]])
+def test_a_trace_records_the_op(op, fp8_without_a_gpu):
+    with torch.no_grad():
+        traced = torch.jit.trace(op, (torch.ones(2, 3),), check_trace=False)
+        assert torch.equal(traced(torch.full((2, 3), 3.0)), torch.full((2, 3), 6.0))
+
+
+def test_without_a_residual_the_sum_is_x_itself(fp8_without_a_gpu):
+    x = torch.ones(2, 3)
+    assert add_rms_norm_fp8(x)[2] is x and add_rms_norm_fp8(x, x)[2] is not x
+    with forward_ad.dual_level():
+        assert add_rms_norm_fp8(x)[2] is x
