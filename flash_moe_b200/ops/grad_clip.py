@@ -72,11 +72,15 @@ def _once(tensors: Iterable[torch.Tensor], what: str) -> List[torch.Tensor]:
         elif t.device != dev:
             _lib.require_cuda(t)
             raise _lib.FmoeError(f"tensors on different devices: {dev} and {t.device}")
+        key = (t.data_ptr(), n, t.dtype)
         if not t.is_contiguous() and not _dense(t):
             if what:
                 raise _lib.FmoeError(what)
+            key += (t.shape, t.stride())  # of the values given, not of their copy
+            if key in seen:
+                continue
             t = t.contiguous()
-        seen.setdefault((t.data_ptr(), n, t.dtype), t)
+        seen.setdefault(key, t)
     return list(seen.values())
 
 

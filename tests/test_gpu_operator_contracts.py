@@ -98,3 +98,12 @@ def test_rows_shorter_than_a_piece(H, dtype):
         w = randn(H, seed=5, dtype=dtype, scale=0.2) + 1
         check_norm(x.detach(), r.detach(), w, randn(T, H, seed=1, dtype=dtype), randn(T, H, seed=2, dtype=dtype))
         assert all(bool(t[T * H :].isnan().all()) for t in whole)
+
+
+def test_norm_of_a_tensor_with_gaps_given_twice():
+    from flash_moe_b200 import grad_norm
+
+    gaps = randn(40, 30, seed=1, dtype=torch.float32)[:, ::2]
+    once = grad_norm(gaps)
+    assert torch.equal(grad_norm([gaps, gaps]), once)
+    assert abs(float(once) - float(gaps.double().norm())) <= 11 * U * float(once)

@@ -6,7 +6,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from flash_moe_b200 import add_rms_norm_fp8
+from flash_moe_b200 import add_rms_norm_fp8, grad_norm
 
 
 @pytest.fixture
@@ -43,3 +43,22 @@ def test_without_a_residual_the_sum_is_x_itself(fp8_without_a_gpu):
     assert add_rms_norm_fp8(x)[2] is x and add_rms_norm_fp8(x, x)[2] is not x
     with forward_ad.dual_level():
         assert add_rms_norm_fp8(x)[2] is x
+
+
+@pytest.fixture
+def clip_without_a_gpu(monkeypatch):
+    """Collects what the library would be given."""
+    given = []
+    clip = sys.modules["flash_moe_b200.ops.grad_clip"]
+    monkeypatch.setattr(clip._lib, "require_cuda", lambda *t: t[0].device)
+    monkeypatch.setattr(clip, "_call", lambda name, grads, head, scale: given.append((name, grads)) or torch.zeros(()))
+    return given
+
+
+def test_a_tensor_with_gaps_given_twice_counts_once(clip_without_a_gpu):
+    base = torch.arange(24.0).view(4, 6)
+    gaps, other, repeated = base[:, ::2], base[:, 1::2], base[:1].expand(4, 6)
+    grad_norm([gaps, base, gaps, other, base[:, ::2], repeated, base, repeated.detach()])
+    ((name, grads),) = clip_without_a_gpu
+    assert name == "fmoe_grad_norm" and [t.flatten().tolist() for t in grads] == [
+        t.flatten().tolist() for t in (gaps, base, other, repeated)]
