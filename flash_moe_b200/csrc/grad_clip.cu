@@ -192,8 +192,8 @@ __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_const
 int grid_cap() { return device_sm_count() * 2; }
 int launches(int count) { return (count + kTensors - 1) / kTensors; }
 
-// no two tensors may share memory: one would be scaled twice
-int check_tensors(void* const* grads, const int64_t* numels, const int32_t* dtypes, int count) {
+// apart: no two tensors may share memory, where they are written: one would be scaled twice
+int check_tensors(void* const* grads, const int64_t* numels, const int32_t* dtypes, int count, bool apart) {
   struct Range {
     uintptr_t lo, hi;
   };
@@ -208,7 +208,7 @@ int check_tensors(void* const* grads, const int64_t* numels, const int32_t* dtyp
       r[n++] = {lo, lo + static_cast<uintptr_t>(numels[i]) * dtype_size(dtypes[i])};
     }
   }
-  if (rc == FMOE_OK) {
+  if (rc == FMOE_OK && apart) {
     std::sort(r, r + n, [](const Range& a, const Range& b) { return a.lo < b.lo; });
     for (int i = 1; i < n; ++i)
       if (r[i].lo < r[i - 1].hi) rc = FMOE_ERR_BAD_ARG;
@@ -251,7 +251,7 @@ int launch_grad_norm(void* const* grads, const int64_t* numels, const int32_t* d
   }
   if (ws == nullptr || ws_bytes < grad_norm_workspace_bytes(count)) return FMOE_ERR_WORKSPACE;
   if (!aligned16(ws)) return FMOE_ERR_ALIGNMENT;
-  const int rc = check_tensors(grads, numels, dtypes, count);
+  const int rc = check_tensors(grads, numels, dtypes, count, clip);
   if (rc != FMOE_OK) return rc;
   double* part = static_cast<double*>(ws);
   int parts = 0;

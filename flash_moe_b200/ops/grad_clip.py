@@ -85,8 +85,8 @@ def _once(tensors: Iterable[torch.Tensor], what: str) -> List[torch.Tensor]:
 
 
 def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], grad_scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
-    """``grad_scale * sqrt(sum of all squares)`` over all tensors, a float32 scalar on their device (no synchronisation).  A tensor
-    given twice counts once."""
+    """``grad_scale * sqrt(sum of all squares)`` over all tensors, a float32 scalar on their device (no synchronisation), as a constant:
+    no graph is recorded through it.  A tensor given twice counts once; of two that overlap, each counts whole."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
     grads = _once((t.detach() for t in tensors), "")
     if not grads:

@@ -229,8 +229,8 @@ int fmoe_add_rms_norm_backward(const void* dnormed, const void* dsummed, const v
  *   fmoe_grad_norm       *norm = scale * sqrt(sum over all values g^2)
  *   fmoe_clip_grad_norm  the same, then in place g <- g * scale * min(1, max_norm / (*norm + eps)); nothing is written where that
  *                        factor is 1.  A norm that is not finite makes the gradients so, or zero them, as the formula says
- * grads, numels and dtypes are HOST arrays of num_tensors entries, grads device pointers to dense tensors of any alignment, no
- * two of which may share memory.  scale >= 0; device_scale (nullable, one float in device memory) multiplies it: the inverse of
+ * grads, numels and dtypes are HOST arrays of num_tensors entries, grads device pointers to dense tensors of any alignment; no
+ * two that are clipped may share memory.  scale >= 0; device_scale (nullable, one float in device memory) multiplies it: the inverse of
  * a loss scale.  Squares and products in float32, the sum over 32 KiB pieces in float64, in a fixed order.  The workspace is
  * 16-byte aligned.
  */

@@ -107,3 +107,14 @@ def test_norm_of_a_tensor_with_gaps_given_twice():
     once = grad_norm(gaps)
     assert torch.equal(grad_norm([gaps, gaps]), once)
     assert abs(float(once) - float(gaps.double().norm())) <= 11 * U * float(once)
+
+
+def test_norm_of_tensors_that_overlap():
+    """Nothing is written, so nothing is refused: each counts whole.  No graph goes through the norm."""
+    from flash_moe_b200 import grad_norm
+
+    flat = randn(100, seed=2, dtype=torch.float32).requires_grad_()
+    parts = [flat[:60], flat[40:], flat.detach()[30:70]]
+    got = grad_norm(parts)
+    want = sum(float(p.detach().double().square().sum()) for p in parts) ** 0.5
+    assert not got.requires_grad and abs(float(got) - want) <= 11 * U * want
