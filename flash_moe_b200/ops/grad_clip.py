@@ -10,6 +10,7 @@ from typing import Iterable, List, Union
 import torch
 
 from .. import _lib
+from .utils import refuse_tangents
 
 
 def _dense(t: torch.Tensor) -> bool:
@@ -88,6 +89,7 @@ def grad_norm(tensors: Union[torch.Tensor, Iterable[torch.Tensor]], grad_scale: 
     """``grad_scale * sqrt(sum of all squares)`` over all tensors, a float32 scalar on their device (no synchronisation), as a constant:
     no graph is recorded through it.  A tensor given twice counts once; of two that overlap, each counts whole."""
     tensors = [tensors] if isinstance(tensors, torch.Tensor) else list(tensors)
+    refuse_tangents("grad_norm", tensors)
     grads = _once((t.detach() for t in tensors), "")
     if not grads:
         return torch.zeros((), device=tensors[0].device if tensors else None)
@@ -109,8 +111,9 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0:
         raise _lib.FmoeError("max_norm and eps must not be negative")
-    grads = _once([g for g in [p.grad for p in parameters] if g is not None],
-                  "a gradient with gaps or repeated values cannot be scaled in place: make it contiguous")
+    grads = [g for g in [p.grad for p in parameters] if g is not None]
+    refuse_tangents("clip_grad_norm_", grads)
+    grads = _once(grads, "a gradient with gaps or repeated values cannot be scaled in place: make it contiguous")
     if not grads:
         return torch.zeros((), device=parameters[0].device if parameters else None)
     norm = _call("fmoe_clip_grad_norm", grads, (max_norm, eps), grad_scale)

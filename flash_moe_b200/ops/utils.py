@@ -5,6 +5,8 @@ from __future__ import annotations
 import torch
 from torch.autograd import forward_ad
 
+from .._lib import FmoeError
+
 
 def contiguous(t):
     """The reference makes every tensor argument contiguous before a kernel sees it (ops/utils.py:35-45)."""
@@ -24,6 +26,12 @@ def plain_call() -> bool:
 def plain_call_without_gradient() -> bool:
     """The same for an op that has no gradient, whatever the grad mode."""
     return forward_ad._current_level < 0 and not _tracing()
+
+
+def refuse_tangents(name, tensors):
+    """For what has no autograd node to refuse them."""
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise FmoeError(f"{name} has no forward-mode derivative (jvp)")
 
 
 def backward_once(backward):

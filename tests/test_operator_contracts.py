@@ -6,7 +6,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from flash_moe_b200 import add_rms_norm_fp8, grad_norm
+from flash_moe_b200 import FmoeError, add_rms_norm_fp8, clip_grad_norm_, grad_norm
 
 
 @pytest.fixture
@@ -62,3 +62,20 @@ def test_a_tensor_with_gaps_given_twice_counts_once(clip_without_a_gpu):
     ((name, grads),) = clip_without_a_gpu
     assert name == "fmoe_grad_norm" and [t.flatten().tolist() for t in grads] == [
         t.flatten().tolist() for t in (gaps, base, other, repeated)]
+
+
+def test_norms_refuse_tangents(clip_without_a_gpu):
+    plain = torch.nn.Parameter(torch.ones(3))
+    plain.grad = torch.ones(3)
+    with torch.no_grad(), forward_ad.dual_level():
+        dual = forward_ad.make_dual(torch.ones(3), torch.ones(3))
+        with pytest.raises(FmoeError, match="jvp"):
+            grad_norm([torch.ones(2), dual])
+        p = torch.nn.Parameter(torch.ones(3))
+        p.grad = dual
+        with pytest.raises(FmoeError, match="jvp"):
+            clip_grad_norm_([plain, p], 1.0)
+        assert not clip_without_a_gpu
+        grad_norm(torch.ones(2))  # a level alone is no tangent
+        clip_grad_norm_(plain, 1.0)
+    assert len(clip_without_a_gpu) == 2
