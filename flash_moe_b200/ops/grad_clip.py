@@ -25,6 +25,11 @@ def _dense(t: torch.Tensor) -> bool:
     return True
 
 
+def _share_memory(dense: List[torch.Tensor]) -> bool:
+    spans = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()) for t in dense)
+    return any(a[1] > b[0] for a, b in zip(spans, spans[1:]))
+
+
 def _call(name, grads: List[torch.Tensor], head, grad_scale) -> torch.Tensor:
     dev = grads[0].device
     scale, device_scale = grad_scale, None
@@ -48,7 +53,7 @@ def _call(name, grads: List[torch.Tensor], head, grad_scale) -> torch.Tensor:
     ws = grads[0].new_empty(nbytes, dtype=torch.uint8)
     rc = _lib.call(name, dev, ptrs.buffer_info()[0], numels.buffer_info()[0], codes.buffer_info()[0], n, *head, scale, device_scale,
                    norm.data_ptr(), ws.data_ptr(), nbytes)
-    if rc == _lib.ERR_BAD_ARG:
+    if rc == _lib.ERR_BAD_ARG and _share_memory(grads):
         raise _lib.FmoeError("two gradients share memory")
     if rc:
         _lib.check(rc, name)

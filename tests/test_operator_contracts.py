@@ -79,3 +79,20 @@ def test_norms_refuse_tangents(clip_without_a_gpu):
         grad_norm(torch.ones(2))  # a level alone is no tangent
         clip_grad_norm_(plain, 1.0)
     assert len(clip_without_a_gpu) == 2
+
+
+def test_a_refused_argument_is_not_called_shared_memory(monkeypatch):
+    """The library has one code for arguments that it refuses; only gradients that do share memory are said to."""
+    clip = sys.modules["flash_moe_b200.ops.grad_clip"]
+    monkeypatch.setattr(clip._lib, "require_cuda", lambda *t: t[0].device)
+    monkeypatch.setattr(clip, "_workspace_bytes", lambda n: 8)
+    monkeypatch.setattr(clip._lib, "call", lambda *a: clip._lib.ERR_BAD_ARG)
+    a, b = (torch.nn.Parameter(torch.zeros(6)) for _ in range(2))
+    flat = torch.ones(12)
+    a.grad, b.grad = flat[:6], flat[6:]
+    with pytest.raises(FmoeError, match="code 1") as e:
+        clip_grad_norm_([a, b], 1.0)
+    assert "share" not in str(e.value)
+    b.grad = flat[5:11]
+    with pytest.raises(FmoeError, match="share memory"):
+        clip_grad_norm_([b, a], 1.0)
