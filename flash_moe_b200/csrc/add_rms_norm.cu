@@ -574,10 +574,11 @@ template <int N> int smallest_shape(const Shape (&shapes)[N], int pieces) {
 int shape_of(bool vec, int pieces) { return vec ? smallest_shape(kVecShapes, pieces) : smallest_shape(kOneShapes, pieces); }
 
 // Groups that the grid of a backward has: all that its registers let run at once, and no more, since each group leaves a row of
-// partial sums.  A multiple of eight, so that SHIFT keeps its remainders.
+// partial sums.  A multiple of eight, so that SHIFT keeps its remainders.  The device has no say: the workspace may have been sized
+// while another was current.
 int64_t backward_groups(Shape sh, int64_t rows) {
   const int cta = sh.wpg < 8 ? 256 : 32 * sh.wpg, per_cta = cta / (32 * sh.wpg);
-  const int64_t cap = static_cast<int64_t>(device_sm_count()) * (sh.wpg * sh.c <= 16 ? 2 : 1) * per_cta / 8 * 8;
+  const int64_t cap = static_cast<int64_t>(kB200Sms) * (sh.wpg * sh.c <= 16 ? 2 : 1) * per_cta / 8 * 8;
   return rows < cap ? (rows + 7) / 8 * 8 : cap;
 }
 

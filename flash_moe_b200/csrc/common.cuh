@@ -32,6 +32,8 @@ inline int next_pow2(int v) {
 }
 
 int device_sm_count();  // cached per device (api.cu)
+// SMs of a B200: for grids that decide how large a workspace is, which is asked for without a device
+constexpr int kB200Sms = 148;
 
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) and the occupancy query cost a microsecond or more each, in front of
 // every launch: both remember what they did per host thread, device and kernel (api.cu).

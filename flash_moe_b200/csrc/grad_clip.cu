@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_const
   }
 }
 
-int grid_cap() { return device_sm_count() * 2; }
+constexpr int kGridCap = kB200Sms * 2;  // whatever the device: the workspace may have been sized while another was current
 int launches(int count) { return (count + kTensors - 1) / kTensors; }
 
 // apart: no two tensors may share memory, where they are written: one would be scaled twice
@@ -231,13 +231,13 @@ void fill(TensorList* l, void* const* grads, const int64_t* numels, const int32_
 
 int grid_of(const TensorList& l) {
   const int64_t chunks = l.first[l.count];
-  return static_cast<int>(chunks < 1 ? 1 : chunks < grid_cap() ? chunks : grid_cap());
+  return static_cast<int>(chunks < 1 ? 1 : chunks < kGridCap ? chunks : kGridCap);
 }
 
 }  // namespace
 
 size_t grad_norm_workspace_bytes(int count) {
-  return count <= 0 ? 0 : static_cast<size_t>(launches(count)) * grid_cap() * sizeof(double);
+  return count <= 0 ? 0 : static_cast<size_t>(launches(count)) * kGridCap * sizeof(double);
 }
 
 int launch_grad_norm(void* const* grads, const int64_t* numels, const int32_t* dtypes, int count, bool clip, float max_norm,

@@ -96,3 +96,14 @@ def test_a_refused_argument_is_not_called_shared_memory(monkeypatch):
     b.grad = flat[5:11]
     with pytest.raises(FmoeError, match="share memory"):
         clip_grad_norm_([b, a], 1.0)
+
+
+def test_workspaces_have_one_size_on_every_device():
+    """Sizes are kept per shape, whatever device was current when they were asked for: those of a B200's 148 SMs, here as on a GPU."""
+    from flash_moe_b200 import _lib, build
+
+    build.build()
+    lib = _lib.lib()
+    assert lib.fmoe_grad_norm_workspace_bytes(96) == 2 * 148 * 8 and lib.fmoe_grad_norm_workspace_bytes(97) == 2 * 2 * 148 * 8
+    # two CTAs an SM of two groups each, a float32 row of sums a group
+    assert lib.fmoe_add_rms_norm_backward_workspace_bytes(1 << 20, 2048, 1) == 2 * 2 * 148 * 2048 * 4
