@@ -44,10 +44,12 @@ class FlashMoEStack(nn.Module):
     def forward(self, hidden_states: torch.Tensor, return_routing: bool = False) -> Tuple[torch.Tensor, List[torch.Tensor]]:
         """Returns the final hidden states and every layer's router logits.  ``return_routing=True`` keeps every layer's
         selected ids and gates in its ``last_indices`` / ``last_gates``."""
+        # handed on only where it is asked for: a layer that a caller put here may not know it
+        routing = {"return_routing": True} if return_routing else {}
         if self.norms is not None and self.fused_norm and torch.is_grad_enabled() and not torch.is_autocast_enabled("cuda") \
                 and all(w.dtype == hidden_states.dtype for w in self.norms) \
                 and (hidden_states.requires_grad or any(p.requires_grad for p in self.parameters())):
-            return self._forward_fused_norm(hidden_states, return_routing)
+            return self._forward_fused_norm(hidden_states, routing)
         all_logits = []
         x = hidden_states
         for i, layer in enumerate(self.layers):
@@ -58,13 +60,13 @@ class FlashMoEStack(nn.Module):
                     from ..ops.rms_norm import rms_norm
 
                     xn = rms_norm(x, self.norms[i].detach(), self.norm_eps)
-                x, logits = layer(xn, return_routing=return_routing, residual=x)
+                x, logits = layer(xn, residual=x, **routing)
             else:
-                x, logits = layer(x, return_routing=return_routing, residual=x)
+                x, logits = layer(x, residual=x, **routing)
             all_logits.append(logits)
         return x, all_logits
 
-    def _forward_fused_norm(self, x, return_routing):
+    def _forward_fused_norm(self, x, routing):
         from ..ops.add_rms_norm import add_rms_norm
 
         all_logits, y = [], None
@@ -73,7 +75,7 @@ class FlashMoEStack(nn.Module):
                 xn, x = add_rms_norm(x, None, weight, self.norm_eps)
             else:
                 xn, x = add_rms_norm(y, x, weight, self.norm_eps)
-            y, logits = layer(xn, return_routing=return_routing)
+            y, logits = layer(xn, **routing)
             all_logits.append(logits)
         return (x if y is None else x + y), all_logits
 

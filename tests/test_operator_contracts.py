@@ -107,3 +107,27 @@ def test_workspaces_have_one_size_on_every_device():
     assert lib.fmoe_grad_norm_workspace_bytes(96) == 2 * 148 * 8 and lib.fmoe_grad_norm_workspace_bytes(97) == 2 * 2 * 148 * 8
     # two CTAs an SM of two groups each, a float32 row of sums a group
     assert lib.fmoe_add_rms_norm_backward_workspace_bytes(1 << 20, 2048, 1) == 2 * 2 * 148 * 2048 * 4
+
+
+class OwnLayer(torch.nn.Module):
+    """What a caller may put in a stack's place of a layer: it takes the states and a residual, no more."""
+
+    def forward(self, x, residual=None):
+        return 2 * x if residual is None else residual + 2 * x, x.detach()
+
+
+@pytest.mark.parametrize("pre_norm,fused_norm", [(False, False), (True, False), (True, True)])
+def test_layers_of_a_stack_that_know_no_routing(pre_norm, fused_norm, monkeypatch):
+    from flash_moe_b200 import FlashMoEConfig
+    from flash_moe_b200.modules.stack import FlashMoEStack
+
+    norm = sys.modules["flash_moe_b200.ops.add_rms_norm"]
+    monkeypatch.setattr(norm, "add_rms_norm", lambda x, r, w, eps: (x * w, x) if r is None else ((x + r) * w, x + r))
+    monkeypatch.setattr(torch.nn.functional, "rms_norm", lambda x, shape, w, eps: x * w)
+    stack = FlashMoEStack(FlashMoEConfig(16, 16, "silu", 16, 2), 2, pre_norm=pre_norm, fused_norm=fused_norm)
+    stack.layers[0], stack.layers[1] = OwnLayer(), OwnLayer()
+    x = torch.ones(1, 2, 16, requires_grad=True)
+    y, logits = stack(x)
+    assert torch.equal(y, torch.full_like(y, 9.0)) and len(logits) == 2
+    with pytest.raises(TypeError, match="return_routing"):
+        stack(x, return_routing=True)
