@@ -77,6 +77,8 @@ class StageTimer:
 
 
 class FlashMoE(nn.Module):
+    _routed_last = False  # whether the last forward kept last_indices; of the class, for modules that were pickled without it
+
     def __init__(self, config: FlashMoEConfig, overlap_shared_mlp: bool = False):
         super().__init__()
         self.hidden_size = config.hidden_size
@@ -183,14 +185,22 @@ class FlashMoE(nn.Module):
             self.last_indices, self.last_gates = indices, gates.detach()
         return (shared + experts).view(bsz, seq_len, -1), router_logits
 
+    def _keep_ids(self, router_logits: torch.Tensor) -> None:
+        """The logits that a forward with ``return_routing=True`` returns carry the ids that it selected: `balance_loss` counts
+        these whatever forwards came in between."""
+        router_logits.selected_experts = self.last_indices
+        self._routed_last = True
+
     def balance_loss(self, router_logits: torch.Tensor, token_mask: Optional[torch.Tensor] = None) -> torch.Tensor:
         """`flash_moe_b200.balance_loss` of the logits that a forward with ``return_routing=True`` returned, with the counts of
-        the ids that it selected (``last_indices``; call it before the next such forward)."""
+        the ids that this forward selected.  Logits made of those (cast, detached, passed through a wrapper) go with the ids of
+        the last forward, which has to be the one that they come from."""
         from ..ops.balance import balance_loss, expert_counts
 
-        if self.last_indices is None or router_logits.dim() != 3 or self.last_indices.shape[0] != router_logits.shape[1]:
-            raise _lib.FmoeError("balance_loss needs the logits of the last forward with return_routing=True")
-        return balance_loss(router_logits, expert_counts(self.last_indices, self.num_experts, token_mask), token_mask)
+        indices = getattr(router_logits, "selected_experts", self.last_indices if self._routed_last else None)
+        if indices is None or router_logits.dim() != 3 or indices.shape[0] != router_logits.shape[1]:
+            raise _lib.FmoeError("balance_loss needs the logits of a forward with return_routing=True, or of the last forward made with it")
+        return balance_loss(router_logits, expert_counts(indices, self.num_experts, token_mask), token_mask)
 
     def clip_grad_norm_(self, max_norm: float, grad_scale: Union[float, torch.Tensor] = 1.0) -> torch.Tensor:
         """`flash_moe_b200.clip_grad_norm_` for the parameters of the layer."""
@@ -233,6 +243,10 @@ class FlashMoE(nn.Module):
             if bn_sync_group is not None or stage_timer is not None:
                 raise _lib.FmoeError("bn_sync_group and stage_timer belong to the fused path: call under torch.no_grad()")
             y, router_logits = self._forward_differentiable(hidden_states, return_routing)
+            if return_routing:
+                self._keep_ids(router_logits)
+            elif self._routed_last:
+                self._routed_last = False
             return (y if residual is None else residual + y), router_logits
         x = hidden_states if hidden_states.is_contiguous() else hidden_states.contiguous()
         dtype = x.dtype
@@ -312,9 +326,13 @@ class FlashMoE(nn.Module):
         # input, the outputs and the workspace need no cross-stream bookkeeping afterwards.
         if training and self.training and bn.num_batches_tracked is not None:
             bn.num_batches_tracked += 1
+        logits = logits.transpose(0, 1)
         if return_routing:
             self.last_indices, self.last_gates = idx, gates
-        return y, logits.transpose(0, 1)
+            self._keep_ids(logits)
+        elif self._routed_last:
+            self._routed_last = False
+        return y, logits
 
 
 class GraphedFlashMoE:

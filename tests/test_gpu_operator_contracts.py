@@ -118,3 +118,24 @@ def test_norm_of_tensors_that_overlap():
     got = grad_norm(parts)
     want = sum(float(p.detach().double().square().sum()) for p in parts) ** 0.5
     assert not got.requires_grad and abs(float(got) - want) <= 11 * U * want
+
+
+def test_two_forwards_before_their_losses():
+    """Two micro-batches of one size, one of them without a graph: each loss has the ids of its own forward."""
+    from flash_moe_b200 import FlashMoE, FlashMoEConfig, FmoeError, balance_loss, expert_counts
+
+    torch.manual_seed(0)
+    layer = FlashMoE(FlashMoEConfig(64, 64, "silu", 256, 4)).cuda().train()
+    a, b = (torch.randn(1, 50, 64, device="cuda") for _ in range(2))
+    logits_a = layer(a, return_routing=True)[1]
+    ids_a = layer.last_indices.clone()
+    with torch.no_grad():
+        logits_b = layer(b, return_routing=True)[1]
+    ids_b = layer.last_indices.clone()
+    assert not torch.equal(ids_a, ids_b)
+    for logits, ids in ((logits_a, ids_a), (logits_b, ids_b)):
+        assert torch.equal(layer.balance_loss(logits), balance_loss(logits, expert_counts(ids, 256)))
+    (grad,) = torch.autograd.grad(layer.balance_loss(logits_a), layer.router_gate.weight)
+    assert bool((grad != 0).any())
+    with pytest.raises(FmoeError, match="return_routing"):
+        layer.balance_loss(layer(a)[1])

@@ -131,3 +131,49 @@ def test_layers_of_a_stack_that_know_no_routing(pre_norm, fused_norm, monkeypatc
     assert torch.equal(y, torch.full_like(y, 9.0)) and len(logits) == 2
     with pytest.raises(TypeError, match="return_routing"):
         stack(x, return_routing=True)
+
+
+@pytest.fixture
+def layer_without_a_gpu(monkeypatch):
+    """A layer whose forwards select expert 1, 2, 3, ... for every token, and whose loss says what it was given."""
+    from flash_moe_b200 import FlashMoE, FlashMoEConfig
+    from flash_moe_b200.modules import flash_moe
+
+    layer = FlashMoE(FlashMoEConfig(16, 16, "silu", 16, 2))
+    calls = []
+
+    def forward(x, return_routing=False):
+        calls.append(return_routing)
+        if return_routing:
+            layer.last_indices, layer.last_gates = torch.full((x.shape[1], 2), len(calls)), torch.ones(x.shape[1], 2)
+        return x, torch.zeros(x.shape[1], 2, 4, requires_grad=True).transpose(0, 1)
+
+    balance = sys.modules["flash_moe_b200.ops.balance"]
+    monkeypatch.setattr(flash_moe._lib, "require_cuda", lambda *t: None)
+    monkeypatch.setattr(layer, "_forward_differentiable", forward)
+    monkeypatch.setattr(balance, "expert_counts", lambda indices, n, mask: indices)
+    monkeypatch.setattr(balance, "balance_loss", lambda logits, counts, mask: int(counts[0, 0]))
+    return layer
+
+
+def test_balance_loss_counts_the_ids_of_its_logits(layer_without_a_gpu):
+    layer, x = layer_without_a_gpu, torch.ones(1, 3, 16)
+    first, second = (layer(x, return_routing=True)[1] for _ in range(2))
+    assert [layer.balance_loss(t) for t in (first, second, first)] == [1, 2, 1]
+    assert layer.balance_loss(second.detach().double()) == 2  # of the last forward
+    layer(x)
+    assert layer.balance_loss(first) == 1 and torch.equal(layer.last_indices, torch.full((3, 2), 2))
+
+
+def test_balance_loss_refuses_logits_without_ids(layer_without_a_gpu):
+    layer, x = layer_without_a_gpu, torch.ones(1, 3, 16)
+    with pytest.raises(FmoeError, match="return_routing"):
+        layer.balance_loss(layer(x)[1])
+    routed = layer(x, return_routing=True)[1]
+    with pytest.raises(FmoeError, match="return_routing"):  # as many tokens, but the ids are another forward's
+        layer.balance_loss(layer(x)[1])
+    with pytest.raises(FmoeError, match="return_routing"):
+        layer.balance_loss(routed.detach())
+    layer(x, return_routing=True)
+    with pytest.raises(FmoeError):
+        layer.balance_loss(routed[:, :2])
