@@ -24,6 +24,8 @@ from .flash_moe import FlashMoE, FlashMoEConfig
 
 
 class FlashMoEStack(nn.Module):
+    fused_norm = False  # of the class, for stacks that were pickled without it
+
     def __init__(self, config: FlashMoEConfig, num_layers: int, seeds=None, pre_norm: bool = False, norm_eps: float = 1e-6,
                  fused_norm: bool = False):
         super().__init__()

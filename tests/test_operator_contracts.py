@@ -177,3 +177,17 @@ def test_balance_loss_refuses_logits_without_ids(layer_without_a_gpu):
     layer(x, return_routing=True)
     with pytest.raises(FmoeError):
         layer.balance_loss(routed[:, :2])
+
+
+def test_modules_pickled_without_the_newer_attributes(layer_without_a_gpu, monkeypatch):
+    """nn.Module comes back with the attributes that it had."""
+    from flash_moe_b200 import FlashMoEConfig
+    from flash_moe_b200.modules.stack import FlashMoEStack
+
+    monkeypatch.setattr(torch.nn.functional, "rms_norm", lambda x, shape, w, eps: x * w)
+    stack = FlashMoEStack(FlashMoEConfig(16, 16, "silu", 16, 2), 1, pre_norm=True)
+    stack.layers[0] = OwnLayer()
+    stack.__dict__.pop("fused_norm")
+    assert torch.equal(stack(torch.ones(1, 2, 16, requires_grad=True))[0], torch.full((1, 2, 16), 3.0))
+    layer_without_a_gpu.__dict__.pop("_routed_last", None)
+    layer_without_a_gpu(torch.ones(1, 3, 16))
