@@ -87,7 +87,7 @@ def choose_hot_experts(indices: torch.Tensor, num_experts: int, count: int, grou
     if indices.is_cuda:  # without the host's wait for the size of indices[valid]
         from .ops.balance import expert_counts
 
-        hist = expert_counts(torch.where(valid, indices, -1).reshape(-1, 1), num_experts)
+        hist = expert_counts(torch.where(valid, indices.to(torch.int64), -1).reshape(-1, 1), num_experts)
     else:
         hist = torch.bincount(indices[valid].reshape(-1), minlength=num_experts).to(torch.int64)
     if dist.is_initialized() and dist.get_world_size(group) > 1:

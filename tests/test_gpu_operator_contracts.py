@@ -139,3 +139,19 @@ def test_two_forwards_before_their_losses():
     assert bool((grad != 0).any())
     with pytest.raises(FmoeError, match="return_routing"):
         layer.balance_loss(layer(a)[1])
+
+
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.int16, torch.int32, torch.int64])
+def test_hot_experts_of_ids_of_any_integers(dtype):
+    """Ids that are no expert's count for nobody and are not reported: unsigned bytes have no -1 to put in their place."""
+    from flash_moe_b200 import read_status
+    from flash_moe_b200.parallel import choose_hot_experts
+
+    ids = (torch.arange(300) % 7).view(60, 5).to(dtype)
+    ids[::3, 1] = 120
+    read_status()
+    got = choose_hot_experts(ids.cuda(), 100, 3)
+    assert read_status() == 0
+    # experts with equal counts may take each other's place, so what has to agree is how often the chosen ones were selected
+    seen = torch.bincount(ids.long().reshape(-1), minlength=100)[:100]
+    assert torch.equal(seen[got.cpu()].sort().values, seen[choose_hot_experts(ids, 100, 3)].sort().values)
