@@ -8,9 +8,13 @@
 // The rows of p sum to 1, so a constant taken off C shifts G_h and s_t alike: C is used without its (whole) mean, which keeps
 // the bits of the differences where the counts are nearly even.
 //
-// The two products run on the tensor cores (tcgen05) with float16 operands.  A float16 holds 11 bits: each probability, times 2^15,
-// is the sum of two of them to within 2^-24 of it, and so is a count (exactly up to 2^22; up to 2048 the second is zero and its
-// product is left out).  hi C_hi + lo C_hi + hi C_lo in one float32 accumulator is what a float32 product would give.
+// The two products run on the tensor cores (tcgen05) with float16 operands.  A float16 holds 11 bits, and none below 2^-24, so:
+//   a probability p, times 2^15, is the sum of two of them to within 2^-23 of it, or 2^-40 in all where p < 2^-17; p < 2^-40 is 0;
+//   a count, less the mean, is such a sum exactly up to 2^22 (up to 2048 the second is zero and its product is left out), above
+//   to within 2^-23 of it, or 2^-39 of the largest.
+// hi C_hi + lo C_hi + hi C_lo, without lo C_lo, less than 2^-22 p C, in one float32 accumulator is what a float32 product would give,
+// but for the absolute 2^-40 C a key: where only experts that improbable were selected, of counts whose rounded mean is 0, the loss
+// and what it would pull on are below 2^-40 nk^2 and are not told from 0.  Pieces of bfloat16 would keep them, five products instead of two.
 //
 // Launches: row statistics (maximum and 1 / sum of both halves) beside the sums of the counts; the centred counts as float16
 // pieces in the order in which shared memory wants them; the product with s_t and the loss; for the gradient one more product

@@ -118,7 +118,8 @@ def balance_loss(router_logits: torch.Tensor, counts: torch.Tensor, token_mask: 
     ``router_logits`` is ``[2, T, num_keys]`` as the layer returns it (up to 2048 keys), ``counts`` what `expert_counts` returns
     (its first ``num_keys^2`` entries; ranks that share the tokens all-reduce them first), ``token_mask`` (bool, one for each token,
     False for padding) leaves tokens out of the mean: their logits are not read and their gradient is zero.  The loss is 0 where
-    there is no token or no selection."""
+    there is no token or no selection.  In the sums with the counts each probability is held to 2^-23 of itself, or to 2^-40 where it is
+    below 2^-17."""
     dev = _lib.require_cuda(router_logits, counts)
     if router_logits.dim() != 3 or router_logits.shape[0] != 2 or not 0 < router_logits.shape[2] <= MAX_KEYS:
         raise _lib.FmoeError(f"expected router_logits[2,T,num_keys] with 1 to {MAX_KEYS} keys")

@@ -256,7 +256,8 @@ int fmoe_expert_counts(const int64_t* indices, const uint8_t* token_mask, int64_
  *   *loss = num_keys^2 sum_ij (C_ij / sum C) mean_t p_0[t,i] p_1[t,j],  the mean over the tokens of token_mask (nullable: all);
  *   dlogits [T, 2, num_keys] = its gradient times *upstream (one float in device memory), rows of masked tokens zero.
  * The loss is 0, and so is its gradient, where there is no selection or no token.  Value i of token t and half h of the logits is at
- * logits[t * token_stride + h * half_stride + i].  The forward leaves token_stats (fmoe_balance_loss_stats_floats floats) and
+ * logits[t * token_stride + h * half_stride + i]; rows that start between two 32-bit words are read by the whole words that hold
+ * their values.  Each probability is held to 2^-23 of itself, or to 2^-40 where it is below 2^-17.  The forward leaves token_stats (fmoe_balance_loss_stats_floats floats) and
  * `prepared` for the backward; both and the workspace are 16-byte aligned.  num_keys is at most 2048.
  */
 size_t fmoe_balance_loss_prepared_bytes(int num_keys);

@@ -4,6 +4,7 @@ quotients, rows shorter than a 16-byte piece, weights that start anywhere, tenso
 import pytest
 import torch
 from test_gpu_add_rms_norm import DTYPES, EPS, U, inputs, near, randn, row_u, sum_and_norm
+from test_gpu_balance import logits_of, reference, routing
 
 pytestmark = pytest.mark.gpu
 
@@ -155,3 +156,67 @@ def test_hot_experts_of_ids_of_any_integers(dtype):
     # experts with equal counts may take each other's place, so what has to agree is how often the chosen ones were selected
     seen = torch.bincount(ids.long().reshape(-1), minlength=100)[:100]
     assert torch.equal(seen[got.cpu()].sort().values, seen[choose_hot_experts(ids, 100, 3)].sort().values)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("T,nk,k", [(5, 1001, 3), (3, 1024, 2), (140, 1030, 16), (20, 1537, 4), (9, 2047, 3), (2, 2048, 2), (30, 2048, 8)])
+def test_loss_of_many_keys(T, nk, k, dtype):
+    """Up to the largest number of keys: eight items of 256 columns side by side, sums over 32 blocks; the bounds of
+    test_gpu_balance.py.  Gradients past the largest float16, as this weight of the loss gives where two tokens have 2048 keys, are
+    infinite."""
+    from flash_moe_b200 import balance_loss, expert_counts
+
+    upstream = 2.0**19 if dtype == torch.float16 else 0.01
+    mask = torch.arange(T, device="cuda") % 5 != 0 if T > 100 else None
+    counts = expert_counts(routing(T, nk, k, T), nk * nk, mask)
+    logits = logits_of(T, nk, dtype, T).detach().requires_grad_()
+    loss = balance_loss(logits, counts, mask)
+    (got,) = torch.autograd.grad(loss, logits, torch.tensor(upstream, device="cuda"))
+    want_loss, loss_slack, want, slack = reference(logits, counts, mask, upstream)
+    assert abs(loss.item() - want_loss) <= loss_slack
+    fi = torch.finfo(dtype)
+    over = fi.max * (1 + fi.eps / 4)  # half a step past the largest value, where rounding goes to infinity
+    inf, size = got.isinf(), want.abs()
+    assert bool((inf <= (size + slack >= over)).all()) and bool((~inf <= (size - slack <= over)).all())
+    assert torch.equal(got[inf].sign().double(), want[inf].sign())
+    off = (got.double() - want).abs()
+    assert bool((off <= slack + (size + slack) * fi.eps / 2 + fi.tiny * fi.eps)[~inf].all())
+    if mask is not None:
+        assert bool((got[:, ~mask] == 0).all())
+
+
+@pytest.mark.parametrize("nk", [16, 64, 200])
+@pytest.mark.parametrize("gap", [0.0, 6.0, 11.0, 14.0, 20.0, 26.0, 30.0, 50.0])
+def test_selections_of_improbable_experts_alone(gap, nk):
+    """One expert (3, 5) has all selections, few enough that their mean rounds to 0, and both its keys lie `gap` below the others: no other
+    term covers what is lost of their probabilities, from about 2^-4 / nk down to 0.
+
+    In the units of test_gpu_balance.py, p being off by (nk / 32 + 16 + |t|) u of itself and its two float16 pieces by 2^-23 of it or 2^-40: G
+    is off by (2 nk + 32 + |t|) u p C + 2^-40 C, the loss by p_0 times as much, a gradient by p (|G| + |s|) own units and p times what G
+    and s are off.  Exponentials below 2^-126 are 0."""
+    from flash_moe_b200 import balance_loss
+
+    T = 40
+    counts = torch.zeros(nk * nk, dtype=torch.int64, device="cuda")
+    counts[3 * nk + 5] = 4
+    logits = 0.5 * randn(2, T, nk, seed=nk, dtype=torch.float32)
+    logits[0, :, 3] -= gap
+    logits[1, :, 5] -= gap
+    logits.requires_grad_()
+    loss = balance_loss(logits, counts)
+    (got,) = torch.autograd.grad(loss, logits)
+    x = logits.detach().double()
+    p, c = torch.softmax(x, -1), counts.double().view(nk, nk)
+    G = torch.stack([p[1] @ c.t(), p[0] @ c])
+    s = (p[0] * G[0]).sum(-1)
+    scale = nk * nk / 4 / T
+    t = x.amax(-1, keepdim=True) - x
+    unit, lost = (2 * nk + 32 + 2 * (gap + 4)) * U, torch.stack([c.sum(1), c.sum(0)])[:, None] * 2.0**-40
+    s_off = unit * s + (p[0] * lost[0]).sum(-1)
+    want = scale * p * (G - s[None, :, None])
+    slack = scale * (p * (unit * G + lost + s_off[None, :, None] + t * U * (G + s[None, :, None])) + 2.0**-126 * (G + s[None, :, None] + lost))
+    assert abs(loss.item() - scale * float(s.sum())) <= scale * float(s_off.sum()) + U * scale * float(s.sum())
+    off, bound = (got.double() - want).abs(), slack + (want.abs() + slack) * U + 2.0**-149
+    assert bool((off <= bound).all()), float((off - bound).max())
+    if gap <= 6:  # here the bounds are relative ones
+        assert float((off / want.abs().clamp(min=1e-30)).max()) < 1e-3
