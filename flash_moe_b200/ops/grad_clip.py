@@ -111,7 +111,8 @@ def clip_grad_norm_(parameters: Union[torch.Tensor, Iterable[torch.Tensor]], max
     the inverse of a loss scale, or the number of ranks where averaged gradients are to be summed.  Parameters without a gradient
     are left out, one given twice counts once.  float32, bfloat16 and float16 gradients may be mixed; each must be dense, all on
     one device, and no two may share a part of their memory.  The norm is that of the gradients given: ranks that hold different
-    parameters combine their `grad_norm`s first."""
+    parameters all-reduce the squares of their `grad_norm`s first and scale by the common factor, `max_norm=inf` and `grad_scale =
+    min(1, max_norm / (n + eps))` as a tensor."""
     parameters = [parameters] if isinstance(parameters, torch.Tensor) else list(parameters)
     max_norm, eps = float(max_norm), float(eps)
     if not max_norm >= 0 or not eps >= 0:

@@ -220,3 +220,26 @@ def test_selections_of_improbable_experts_alone(gap, nk):
     assert bool((off <= bound).all()), float((off - bound).max())
     if gap <= 6:  # here the bounds are relative ones
         assert float((off / want.abs().clamp(min=1e-30)).max()) < 1e-3
+
+
+def test_clipping_by_a_norm_that_ranks_share():
+    """Ranks that hold different parameters add up the squares of their norms and scale by the common factor: the gradients are those of one
+    rank that holds all.  Norm and factor are off by a few float32 roundings more than that rank's."""
+    from flash_moe_b200 import clip_grad_norm_, grad_norm
+
+    def rank(seed):
+        params = [torch.nn.Parameter(torch.zeros(n, device="cuda")) for n in (300, 7)]
+        for i, p in enumerate(params):
+            p.grad = randn(p.numel(), seed=seed + i, dtype=torch.float32)
+        return params
+
+    for max_norm in (1.0, 1e3):
+        one = [*rank(1), *rank(5)]
+        norm = clip_grad_norm_(one, max_norm)
+        ranks = [rank(1), rank(5)]
+        total = sum(grad_norm([p.grad for p in r]).square() for r in ranks).sqrt()  # the sum is the all-reduce
+        assert abs(float(total) - float(norm)) <= 32 * U * float(norm)
+        for r in ranks:
+            clip_grad_norm_(r, float("inf"), grad_scale=(max_norm / (total + 1e-6)).clamp(max=1.0))
+        for a, b in zip(one, [*ranks[0], *ranks[1]]):
+            assert bool(((a.grad - b.grad).abs() <= 64 * U * b.grad.abs()).all())
