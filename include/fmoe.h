@@ -213,7 +213,8 @@ int fmoe_rms_norm(const void* x, const void* weight, void* out, int dtype, int64
  *                               (nullable): sums in float32 in a fixed order, one rounding; the workspace, 16-byte
  *                               aligned, is for dweight
  * residual (nullable, then summed is null too: x itself is normalised), weight (nullable) [hidden].  hidden is any number up to
- * 16384, arrays may start anywhere; where they all start at 16 bytes, rows of any length are read in aligned pieces of that size.
+ * 16384, arrays may start anywhere; where all but the weight start at 16 bytes, rows of any length, but for the shortest, are read in
+ * aligned pieces of that size, never past the end of an array.
  */
 int fmoe_add_rms_norm(const void* x, const void* residual, const void* weight, void* summed, void* normed, int dtype,
                       int64_t num_tokens, int hidden, float eps, fmoe_stream_t stream);
